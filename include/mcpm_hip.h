@@ -43,11 +43,14 @@ extern "C" {
 #define MCPM_ERR_FORMAT (-6)      /* malformed GGUF or missing tensor */
 #define MCPM_ERR_NOMEM (-7)       /* device or host allocation failed */
 
-/* ggml tensor type ids, as stored in GGUF. */
+/* ggml tensor type ids, as stored in GGUF.  F16 and BF16 are element types of
+ * the paged cache and its operators only. */
 #define MCPM_TYPE_F32 0
+#define MCPM_TYPE_F16 1
 #define MCPM_TYPE_Q8_0 8
 #define MCPM_TYPE_Q4_K 12
 #define MCPM_TYPE_Q6_K 14
+#define MCPM_TYPE_BF16 30
 
 #define MCPM_QK_K 256
 #define MCPM_Q8K_BYTES 292
@@ -186,6 +189,129 @@ int mcpm_sample_device(mcpm_ctx *ctx, const float *x, int n, float temperature, 
  * call (or since timing was enabled), and starts a new count. */
 int mcpm_set_op_timing(mcpm_ctx *ctx, int enable);
 int mcpm_op_time(mcpm_ctx *ctx, double *total_ms, int64_t *launches);
+
+/* ------------------------------------------- many sequences at once ----- */
+/* No counterpart in the reference, which holds one conversation: for a host
+ * that answers several from one pool of cache pages.  The descriptors are host
+ * structs that a call reads before it returns; the pointers in them are device
+ * memory of the context's GPU.  As the per-op entries, the calls are ordered on
+ * the context's stream and return after enqueueing.  Their scratch belongs to
+ * the context and grows on demand (a call that makes it grow waits for the
+ * stream). */
+
+/* A key-value cache in pages, caller-owned: n_pages pages of page_size (a power
+ * of two up to 65536) positions.  Element (page, position in page, kv head, d)
+ * of k and of v is at page*page_stride + position*pos_stride + head*head_stride
+ * + d, in elements of `type` (F32, F16 or BF16); head_dim is a multiple of 8 up
+ * to 256, k and v are 16-byte aligned and every stride a multiple of 16 bytes.
+ * A contiguous cache [max_seq_len][n_kv_heads][head_dim] is such a pool, its
+ * pages in order.  `weight` (may be NULL): float [n_pages][n_kv_heads][page_size],
+ * the attention each cached position has received. */
+typedef struct {
+    int type;
+    int n_pages, page_size;
+    int n_kv_heads, head_dim;
+    int64_t page_stride, pos_stride, head_stride;
+    void *k, *v;
+    float *weight;
+} mcpm_paged_kv;
+
+/* The sequences of a call.  Position j of sequence b is in page
+ * pages[b*max_pages + j/page_size], at j % page_size; the sequence holds lens[b]
+ * positions, its new tokens included.  Rows starts[b] .. starts[b+1]-1 of q, k, v
+ * and out are its new tokens, the last of its positions, in order (starts:
+ * n_seq+1 ascending row numbers; NULL: row b alone is sequence b's).  n_rows
+ * counts the rows of the buffers (those that no sequence has stay as they are);
+ * max_new and max_len are bounds that the caller gives: no sequence has more new
+ * tokens, or more positions.  Data beyond a bound is never touched: a longer
+ * sequence is taken as one of max_len (or of the positions its table holds),
+ * rows past max_new are left out, and a page number outside the pool's holds
+ * nothing (a position there is neither stored nor seen).  A row whose position
+ * would be negative sees nothing and is not stored. */
+typedef struct {
+    int n_seq, n_rows;
+    int max_new, max_len, max_pages;
+    const int *pages, *lens, *starts;
+} mcpm_paged_batch;
+
+/* What a row at position i sees of position j of its sequence, and how.
+ * score = scale * q.k (scale 0: 1/sqrt(head_dim)); softcap c > 0: c*tanh(score/c);
+ * slopes (float [n_heads]): less slopes[head] * |i - j|.  Seen are j <= i, and j <
+ * prefix[b] also from before (prefix: int [n_seq]); with window > 0 only where
+ * i - j < window; with docs (int [n_seq][docs_stride], docs_stride >= max_len) only
+ * where docs[b][j] == docs[b][i] and that is not negative.  Unset pointers are
+ * NULL.  What is not seen takes no part, whatever it holds; a row that sees
+ * nothing gets zeros. */
+typedef struct {
+    float scale, softcap;
+    int window;
+    const float *slopes;
+    const int *prefix;
+    const int *docs;
+    int64_t docs_stride;
+} mcpm_attn_rules;
+
+/* Stores the new tokens' k and v rows [n_rows][n_kv_heads][head_dim], kv_stride
+ * elements of io_type apart, in their sequences' pages.  With rope_base > 0 the
+ * pairs (2i, 2i+1) of k, and of q rows [n_rows][n_heads][head_dim] (q_stride apart,
+ * in place; NULL: none), are rotated by position * rope_base^(-2i/head_dim) on the
+ * way, the angle in 64 bits (mcpm_apply_rope's is the reference's, in 32).  With
+ * kv->weight the stored positions' weights start at 0.  io_type is F32, or the
+ * cache's type.  Two rows for one position, or pages shared between sequences
+ * that both append, race. */
+int mcpm_paged_append(mcpm_ctx *ctx, const mcpm_paged_kv *kv, const mcpm_paged_batch *batch, int io_type,
+                      const void *k, const void *v, int64_t kv_stride, void *q, int64_t q_stride, int n_heads,
+                      float rope_base);
+
+/* Attention of the rows q [n_rows][n_heads][head_dim] (q_stride apart) over their
+ * sequences' pages (the new tokens' own k and v appended before), into out (same
+ * layout, out_stride apart; memory of its own).  Query head h reads kv head
+ * h / (n_heads/n_kv_heads).  rules may be NULL.  io_type is F32, or the cache's
+ * type.  Sums and the softmax are held in 32 bits; F32 rows over a 16-bit cache
+ * are not rounded to 16 bits.  With kv->weight, each seen position's weight grows
+ * by its share p (they sum to 1 per row and head), summed over the kv head's
+ * query heads and the rows, in an order that does not change from call to call;
+ * sequences that share a page then race. */
+int mcpm_paged_attention(mcpm_ctx *ctx, void *out, int64_t out_stride, const void *q, int64_t q_stride, int io_type,
+                         int n_heads, const mcpm_paged_kv *kv, const mcpm_paged_batch *batch,
+                         const mcpm_attn_rules *rules);
+
+/* Shortens sequences to at most `budget` positions, per kv head: keeps the first
+ * `first`, the last `recent` and, of those between, the ones of the largest weight
+ * (equal ones: the lowest position; NaN counts as less than any), and copies what
+ * is kept, k, v and weight, in order, to positions 0.. of dst_pages (int
+ * [n_seq][max_dst_pages], pages of the same pool that no sequence of the call
+ * uses).  kept (int [n_seq][n_kv_heads][budget]): the positions they had, -1 past
+ * dst_lens[b] = min(lens[b], budget).  kv->weight is required; batch's rows
+ * (starts, n_rows, max_new) are not read.  Kept keys stay rotated by the position
+ * they had. */
+int mcpm_paged_evict(mcpm_ctx *ctx, const mcpm_paged_kv *kv, const mcpm_paged_batch *batch, int budget, int first,
+                     int recent, const int *dst_pages, int max_dst_pages, int *kept, int *dst_lens);
+
+/* Rules on the logits of n_seq sequences, rows of `vocab` floats `stride` apart.
+ * For ids that occur c > 0 times in history[history_starts[b] ..
+ * history_starts[b+1]-1]: l = l > 0 ? l / repetition[b] : l * repetition[b], then
+ * l -= frequency[b]*c + presence[b].  Then l += bias[i] for the ids bias_ids[i], i
+ * from bias_starts[b] to bias_starts[b+1]-1 (an id listed twice: its last entry
+ * counts).  Then -inf where bit (id % 32) of allowed[b*allowed_stride + id/32] is
+ * 0.  Unset pointers are NULL: that rule is left out (history_starts and
+ * bias_starts: int [n_seq+1], ascending; repetition, presence, frequency: float
+ * [n_seq], taken as 1, 0, 0).  Ids outside the vocabulary are passed over. */
+typedef struct {
+    int n_seq, vocab;
+    int64_t stride;
+    const int *history, *history_starts;
+    const float *repetition, *presence, *frequency;
+    const int *bias_ids;
+    const float *bias;
+    const int *bias_starts;
+    const uint32_t *allowed;
+    int64_t allowed_stride;
+} mcpm_logit_rules;
+
+/* Applies the rules in place (before mcpm_argmax or mcpm_sample_device, or the
+ * host's own sampler). */
+int mcpm_process_logits(mcpm_ctx *ctx, float *logits, const mcpm_logit_rules *rules);
 
 /* ------------------------------------------------------------ engine ----- */
 

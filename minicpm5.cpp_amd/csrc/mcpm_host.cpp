@@ -251,6 +251,7 @@ void mcpm_destroy(mcpm_ctx* c) {
   if (c->d_attn_part) (void)hipFree(c->d_attn_part);
   if (c->d_argmax_part) (void)hipFree(c->d_argmax_part);
   if (c->d_sample) (void)hipFree(c->d_sample);
+  if (c->d_paged) (void)hipFree(c->d_paged);
   for (auto& p : c->op_events) {
     (void)hipEventDestroy(p.first);
     (void)hipEventDestroy(p.second);

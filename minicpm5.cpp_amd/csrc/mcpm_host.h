@@ -21,6 +21,8 @@ struct mcpm_ctx {
   int argmax_cap = 0;
   void* d_sample = nullptr;  // device sampler scratch
   size_t sample_cap = 0;
+  void* d_paged = nullptr;  // scratch of the operators over the paged cache
+  size_t paged_cap = 0;
   // per-op kernel timing (mcpm_set_op_timing): an event pair per timed launch
   bool op_timing = false;
   std::vector<std::pair<hipEvent_t, hipEvent_t>> op_events;

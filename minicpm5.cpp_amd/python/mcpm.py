@@ -16,6 +16,7 @@ PKG_DIR = os.path.dirname(_HERE)
 LIB_PATH = os.path.join(PKG_DIR, "libmcpm_hip.so")
 
 TYPE_F32, TYPE_Q8_0, TYPE_Q4_K, TYPE_Q6_K = 0, 8, 12, 14
+TYPE_F16, TYPE_BF16 = 1, 30  # elements of the paged cache and its operators
 KC_QKV, KC_ATTN, KC_OPROJ, KC_GATE_UP, KC_DOWN, KC_LM_HEAD, KC_LAYERS = range(7)
 # mcpm_engine_set_persistent's default mode
 PERSIST_AUTO = 2
@@ -47,6 +48,41 @@ class ModelConfig(C.Structure):
 
     def as_dict(self):
         return {k: getattr(self, k) for k, _ in self._fields_}
+
+
+class PagedKV(C.Structure):
+    """mcpm_paged_kv: a pool of cache pages (k, v, weight: device addresses)."""
+    _fields_ = [
+        ("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int), ("n_kv_heads", C.c_int),
+        ("head_dim", C.c_int), ("page_stride", C.c_int64), ("pos_stride", C.c_int64), ("head_stride", C.c_int64),
+        ("k", C.c_void_p), ("v", C.c_void_p), ("weight", C.c_void_p),
+    ]
+
+
+class PagedBatch(C.Structure):
+    """mcpm_paged_batch: the sequences of a call (pages, lens, starts: device addresses)."""
+    _fields_ = [
+        ("n_seq", C.c_int), ("n_rows", C.c_int), ("max_new", C.c_int), ("max_len", C.c_int), ("max_pages", C.c_int),
+        ("pages", C.c_void_p), ("lens", C.c_void_p), ("starts", C.c_void_p),
+    ]
+
+
+class AttnRules(C.Structure):
+    """mcpm_attn_rules: what a row sees, and how (slopes, prefix, docs: device addresses)."""
+    _fields_ = [
+        ("scale", C.c_float), ("softcap", C.c_float), ("window", C.c_int), ("slopes", C.c_void_p),
+        ("prefix", C.c_void_p), ("docs", C.c_void_p), ("docs_stride", C.c_int64),
+    ]
+
+
+class LogitRules(C.Structure):
+    """mcpm_logit_rules: penalties, biases and allowed ids (device addresses)."""
+    _fields_ = [
+        ("n_seq", C.c_int), ("vocab", C.c_int), ("stride", C.c_int64), ("history", C.c_void_p),
+        ("history_starts", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p),
+        ("frequency", C.c_void_p), ("bias_ids", C.c_void_p), ("bias", C.c_void_p), ("bias_starts", C.c_void_p),
+        ("allowed", C.c_void_p), ("allowed_stride", C.c_int64),
+    ]
 
 
 def make_config(n_layers, dim, n_heads, n_kv_heads, head_dim, ffn, vocab, rope_base=10000.0, eps=1e-6, tied=1):
@@ -109,6 +145,11 @@ _SIGS = {
     "mcpm_get_embedding": (_I, [_P, _P, _P, _I]),
     "mcpm_argmax": (_I, [_P, _P, _I, _P]),
     "mcpm_sample_device": (_I, [_P, _P, _I, _F, _F, _F, _P]),
+    "mcpm_paged_append": (_I, [_P, C.POINTER(PagedKV), C.POINTER(PagedBatch), _I, _P, _P, _I64, _P, _I64, _I, _F]),
+    "mcpm_paged_attention": (_I, [_P, _P, _I64, _P, _I64, _I, _I, C.POINTER(PagedKV), C.POINTER(PagedBatch),
+                                  C.POINTER(AttnRules)]),
+    "mcpm_paged_evict": (_I, [_P, C.POINTER(PagedKV), C.POINTER(PagedBatch), _I, _I, _I, _P, _I, _P, _P]),
+    "mcpm_process_logits": (_I, [_P, _P, C.POINTER(LogitRules)]),
     "mcpm_engine_load_gguf": (_I, [_P, C.c_char_p, C.POINTER(_P)]),
     "mcpm_engine_load_gguf_memory": (_I, [_P, _P, _SZ, C.POINTER(_P)]),
     "mcpm_engine_free": (None, [_P]),
