@@ -203,7 +203,8 @@ int mcpm_op_time(mcpm_ctx *ctx, double *total_ms, int64_t *launches);
  * of two up to 65536) positions.  Element (page, position in page, kv head, d)
  * of k and of v is at page*page_stride + position*pos_stride + head*head_stride
  * + d, in elements of `type` (F32, F16 or BF16); head_dim is a multiple of 8 up
- * to 256, k and v are 16-byte aligned and every stride a multiple of 16 bytes.
+ * to 256, k and v are 16-byte aligned and every stride a multiple of 16 bytes,
+ * pos_stride and head_stride less than 2^31.
  * A contiguous cache [max_seq_len][n_kv_heads][head_dim] is such a pool, its
  * pages in order.  `weight` (may be NULL): float [n_pages][n_kv_heads][page_size],
  * the attention each cached position has received. */

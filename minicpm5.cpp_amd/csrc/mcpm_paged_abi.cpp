@@ -43,6 +43,8 @@ int view_kv(const mcpm_paged_kv* kv, const char* fn, PagedView& out) {
   const int64_t step = 16 / elem_bytes(kv->type);
   for (const int64_t st : {kv->page_stride, kv->pos_stride, kv->head_stride})
     if (st < kv->head_dim || st % step) return fail(MCPM_ERR_ARG, std::string(fn) + ": strides must be multiples of 16 bytes, at least head_dim");
+  if (kv->pos_stride > INT32_MAX || kv->head_stride > INT32_MAX)
+    return fail(MCPM_ERR_ARG, std::string(fn) + ": pos_stride and head_stride must be less than 2^31");
   int shift = 0;
   while ((1 << shift) < kv->page_size) ++shift;
   out = PagedView{static_cast<char*>(kv->k), static_cast<char*>(kv->v), kv->weight, kv->page_stride, kv->pos_stride,
@@ -146,7 +148,7 @@ int mcpm_paged_attention(mcpm_ctx* c, void* out, int64_t out_stride, const void*
   if (!bt.n_seq || !bt.n_rows || !bt.max_new) return MCPM_OK;
   DeviceScope dev(c->device);
   MCPM_HIP(dev.status());
-  rc = ensure_paged_scratch(c, paged_attention_scratch(kvv, bt, n_heads, c->n_cu));
+  rc = ensure_paged_scratch(c, paged_attention_scratch(kvv, bt, rl, n_heads, c->n_cu));
   if (rc) return rc;
   MCPM_HIP(launch_paged_attention(kvv, kv->type, bt, rl, io_type, out, out_stride, q, q_stride, n_heads, c->d_paged, c->n_cu, c->stream));
   return MCPM_OK;

@@ -77,6 +77,8 @@ CACHES = [
     (dict(pos_stride=132), mcpm.ERR_ARG, "strides"),
     (dict(head_stride=56), mcpm.ERR_ARG, "strides"),
     (dict(page_stride=-128), mcpm.ERR_ARG, "strides"),
+    (dict(pos_stride=1 << 31), mcpm.ERR_ARG, "less than 2^31"),
+    (dict(head_stride=1 << 31), mcpm.ERR_ARG, "less than 2^31"),
 ]
 
 
