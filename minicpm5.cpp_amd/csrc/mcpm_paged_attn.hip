@@ -30,103 +30,10 @@ constexpr int FEW_STEP = 32;                // positions of a wave's step
 constexpr int FEW_ROUND = 4 * FEW_STEP;     // of a work group's
 constexpr int FEW_MIN_CHUNK = 256;
 constexpr int FEW_TARGET = 4;               // work groups per CU
+constexpr int PROMPT_TARGET = 1;            // work groups per CU that a prompt's length is split for
+constexpr int PROMPT_MIN_CHUNK = 512;
 constexpr int FEW_MOST = 32;                // new tokens x group up to which these kernels run
 constexpr int FEW_MAX_CHUNK = 2048;         // positions of a work group, at most
-
-struct FewArgs {
-  PagedView kv;
-  BatchView bt;
-  RuleView rl;
-  const void* q;
-  void* out;
-  int64_t q_stride, out_stride;
-  int n_heads, group, n_blocks;  // query heads per kv head; row blocks per (sequence, kv head)
-  int chunk, n_splits;
-  float* part_o;    // [seq][new token][head][split][hd], unnormalised
-  float2* part_mz;  // [seq][new token][head][split]
-  float* scores;    // [seq][kv head][row of the sequence][score_len], or null
-  int score_len, score_rows;
-};
-
-__device__ __forceinline__ int64_t few_part(const FewArgs& a, int b, int t, int head, int split) {
-  return ((static_cast<int64_t>(b) * a.bt.max_new + t) * a.n_heads + head) * a.n_splits + split;
-}
-
-// The positions of a row block.
-struct FewBlock {
-  int r_end;  // rows of the sequence
-  int pos0;   // position of row 0 of the sequence
-  KeyRange keys;
-};
-__device__ __forceinline__ FewBlock few_block(const FewArgs& a, int b, int rb, const SeqRows& sr, int len) {
-  const int pos0 = len - sr.given, r_end = sr.n * a.group;
-  const int t0 = rb * FEW_ROWS / a.group, t1 = (min(rb * FEW_ROWS + FEW_ROWS, r_end) - 1) / a.group;
-  return FewBlock{r_end, pos0, key_range(a.rl, b, pos0 + t0, pos0 + t1, len)};
-}
-
-// Page offsets of a chunk (a page outside the pool stands at the first one, to be masked);
-// whether all of this lane's are in the pool.
-__device__ __forceinline__ bool load_page_offsets(const BatchView& bt, const PagedView& kv, int b, int c0, int c1, int64_t* s_off) {
-  bool ok = true;
-  const int first = c0 >> kv.page_shift, n = ((c1 - 1) >> kv.page_shift) - first + 1;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const int page = page_of(bt, kv, b, (first + i) << kv.page_shift);
-    s_off[i] = page < 0 ? 0 : page * kv.page_stride;
-    ok = ok && page >= 0;
-  }
-  return ok;
-}
-
-// The plain computation of one row over positions [c0, c1), by the whole work
-// group, for values that the matrix products cannot keep apart: a share of 0
-// times what a masked place holds.  Returns this lane's element tid of sum
-// p v, and (m, z).
-template <typename TC, typename TI>
-__device__ __forceinline__ float exact_row(const FewArgs& a, int b, int kh, int row, int head, int pos, int c0, int c1, float* s_q,
-                                        float* s_p, float* s_red, float2* mz) {
-  const PagedView& kv = a.kv;
-  const int tid = threadIdx.x, hd = kv.hd;
-  __syncthreads();
-  if (tid < hd) s_q[tid] = static_cast<float>(static_cast<const TI*>(a.q)[row * a.q_stride + head * hd + tid]);
-  __syncthreads();
-  const ScoreRule sr = score_rule(a.rl);
-  const RowRule rr = row_rule(a.rl, b, pos);
-  const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
-  float m = MAX_START, z = 0.0f, o = 0.0f;
-  for (int j0 = c0; j0 < c1; j0 += 256) {
-    const int j = j0 + tid;
-    float s = -__builtin_inff();
-    const int page = j < c1 && pos >= 0 && seen(a.rl, rr, b, j) ? page_of(a.bt, kv, b, j) : -1;
-    if (page >= 0) {
-      const TC* k = reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh);
-      float d = 0.0f;
-      for (int i = 0; i < hd; ++i) d = __builtin_fmaf(s_q[i], static_cast<float>(k[i]), d);
-      s = score_of(sr, d, sr.mul) - slope * fabsf(static_cast<float>(pos - j));
-    }
-    float w = wave_max(s);
-    if ((tid & 63) == 0) s_red[tid >> 6] = w;
-    __syncthreads();
-    w = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const float mn = fmaxf(m, w), scale = __builtin_amdgcn_exp2f(m - mn);
-    m = mn;
-    s_p[tid] = __builtin_amdgcn_exp2f(s - m);
-    __syncthreads();
-    z *= scale;
-    o *= scale;
-    for (int i = 0; i < min(256, c1 - j0); ++i) {
-      const float p = s_p[i];
-      if (p == 0.0f) continue;
-      z += p;
-      if (tid < hd) {
-        const int pg = page_of(a.bt, kv, b, j0 + i);  // p != 0: in the pool
-        if (pg >= 0) o = __builtin_fmaf(p, static_cast<float>((reinterpret_cast<const TC*>(kv.v) + elem_of(kv, pg, j0 + i, kh))[tid]), o);
-      }
-    }
-    __syncthreads();
-  }
-  *mz = make_float2(m, z);
-  return o;
-}
 
 template <typename TC, typename TI, int DP>
 struct FewTile;
@@ -294,7 +201,7 @@ struct FewTile<float, float, DP> {
 };
 
 template <typename TC, typename TI, int DP>
-__global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
+__global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   __shared__ __attribute__((aligned(16))) float s_o[4][FEW_ROWS][DP + 4];
   __shared__ float s_m[4][FEW_ROWS], s_z[4][FEW_ROWS];
   __shared__ int s_bad;
@@ -307,7 +214,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
   const SeqRows sr = seq_rows(a.bt, b);
   const int len = seq_len(a.bt, kv, b);
   if (rb * FEW_ROWS >= sr.n * a.group) return;
-  const FewBlock fb = few_block(a, b, rb, sr, len);
+  const RowBlock fb = row_block(a, b, rb, sr, len);
   const int c0 = fb.keys.lo + split * a.chunk, c1 = min(fb.keys.hi, c0 + a.chunk);
   if (split && c0 >= fb.keys.hi) return;  // the first one answers for rows that see nothing
 
@@ -340,8 +247,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
   float m = MAX_START, z = 0.0f;
   // Rows of one block differ in position by up to 15 tokens: a step that lies
   // before all of them and inside every window needs no masks.
-  const int pos_min = fb.pos0 + rb * FEW_ROWS / a.group, pos_max = fb.pos0 + (min(rb * FEW_ROWS + FEW_ROWS, fb.r_end) - 1) / a.group;
-  const bool plain = !a.rl.docs && !bad_pages && pos_min >= 0;
+  const bool plain = !a.rl.docs && !bad_pages && fb.first >= 0;
   for (int p0 = c0 + wv * FEW_STEP; p0 < c1; p0 += FEW_ROUND) {
 #pragma unroll
     for (int T = 0; T < 2; ++T) tile.load_k(T, kc + offset(p0 + 16 * T + n16), kv.hd);
@@ -358,7 +264,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i] -= slope * fabsf(static_cast<float>(pos - (p0 + 16 * (i >> 2) + 4 * g + (i & 3))));
     }
-    if (!plain || p0 + FEW_STEP - 1 > pos_min || p0 + FEW_STEP > c1 || (a.rl.window > 0 && pos_max - p0 >= a.rl.window)) {
+    if (!plain || p0 + FEW_STEP - 1 > fb.first || p0 + FEW_STEP > c1 || (a.rl.window > 0 && fb.last - p0 >= a.rl.window)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int j = p0 + 16 * (i >> 2) + 4 * g + (i & 3);
@@ -420,7 +326,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
     Z += w[i] * s_z[i][rn];
   }
   const int64_t rowj = sr.r0 + tj;
-  const int64_t at = few_part(a, b, tj, hj, split);
+  const int64_t at = part_index(a, b, tj, hj, split);
   const bool final = a.n_splits == 1;
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
   TI* dst = static_cast<TI*>(a.out) + rowj * a.out_stride + hj * kv.hd;
@@ -451,7 +357,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const FewArgs a) {
     const int ri = rb * FEW_ROWS + i, ti = ri / a.group, hi = kh * a.group + ri - ti * a.group;
     float2 mz;
     const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + ti, hi, fb.pos0 + ti, c0, c1, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0], &mz);
-    const int64_t ai = few_part(a, b, ti, hi, split);
+    const int64_t ai = part_index(a, b, ti, hi, split);
     if (tid < kv.hd) {
       if (final) static_cast<TI*>(a.out)[(sr.r0 + ti) * a.out_stride + hi * kv.hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
       else a.part_o[ai * kv.hd + tid] = o;
@@ -471,24 +377,23 @@ __device__ __forceinline__ float2 join_mz(const float2* mz, int n) {
   for (int s = 32; s; s >>= 1) Z += __shfl_xor(Z, s);
   return make_float2(M, Z);
 }
-__device__ __forceinline__ int active_splits(const FewArgs& a, const KeyRange& k) {
+__device__ __forceinline__ int active_splits(const PagedCall& a, const KeyRange& k) {
   return k.hi > k.lo ? (k.hi - k.lo + a.chunk - 1) / a.chunk : 1;
 }
 
 // A work group per (new token, head): the splits' partials into the output,
 // 256 / (DP/4) of them at a time.
 template <typename TI, int DP>
-__global__ void __launch_bounds__(256) k_attention_join(const FewArgs a) {
+__global__ void __launch_bounds__(256) k_attention_join(const PagedCall a) {
   constexpr int LP = DP / 4, GR = 256 / LP;
   __shared__ f32x4 s_acc[GR][LP];
   const int b = blockIdx.y, tid = threadIdx.x, hd = a.kv.hd;
   const SeqRows sr = seq_rows(a.bt, b);
   const int t = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads;
   if (t >= sr.n) return;
-  const int rb = (t * a.group + head % a.group) / FEW_ROWS;
-  const FewBlock fb = few_block(a, b, rb, sr, seq_len(a.bt, a.kv, b));
-  const int n = active_splits(a, fb.keys);
-  const int64_t at = few_part(a, b, t, head, 0);
+  const int rb = (t * a.group + head % a.group) / a.block_rows;
+  const int n = active_splits(a, row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b)).keys);
+  const int64_t at = part_index(a, b, t, head, 0);
   const float2 mz = join_mz(a.part_mz + at, n);
   const int d = tid % LP * 4;
   f32x4 acc{0, 0, 0, 0};
@@ -499,6 +404,7 @@ __global__ void __launch_bounds__(256) k_attention_join(const FewArgs a) {
     }
   s_acc[tid / LP][tid % LP] = acc;
   __syncthreads();
+  if (tid == 0 && a.kv.weight) a.part_mz[at] = mz;
   if (tid >= LP || d >= hd) return;
   for (int i = 1; i < GR; ++i) acc += s_acc[i][tid];
   const float inv = mz.y == 0.0f ? 0.0f : 1.0f / mz.y;
@@ -508,7 +414,7 @@ __global__ void __launch_bounds__(256) k_attention_join(const FewArgs a) {
 }
 
 // The positions' weights from the scores: a lane per position sums its rows in order.
-__global__ void __launch_bounds__(256) k_attention_weight(const FewArgs a) {
+__global__ void __launch_bounds__(256) k_attention_weight(const PagedCall a) {
   __shared__ float2 s_mz[FEW_ROWS];
   const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, j = blockIdx.x * 256 + tid;
   const int len = seq_len(a.bt, a.kv, b);
@@ -518,12 +424,12 @@ __global__ void __launch_bounds__(256) k_attention_weight(const FewArgs a) {
   const float* sc = a.scores + (static_cast<int64_t>(b) * a.kv.n_kv_heads + kh) * a.score_rows * a.score_len + j;
   float sum = 0.0f;
   for (int r0 = 0; r0 < rows; r0 += FEW_ROWS) {
-    const FewBlock fb = few_block(a, b, r0 / FEW_ROWS, sr, len);
+    const RowBlock fb = row_block(a, b, r0 / FEW_ROWS, sr, len);
     __syncthreads();
-    for (int i = tid >> 6; i < FEW_ROWS && r0 + i < rows; i += 4) {
-      const int t = (r0 + i) / a.group;
-      const float2 mz = join_mz(a.part_mz + few_part(a, b, t, kh * a.group + r0 + i - t * a.group, 0), active_splits(a, fb.keys));
-      if ((tid & 63) == 0) s_mz[i] = make_float2(mz.x, mz.y == 0.0f ? 0.0f : 1.0f / mz.y);
+    if (tid < FEW_ROWS && r0 + tid < rows) {
+      const int t = (r0 + tid) / a.group;
+      const float2 mz = a.part_mz[part_index(a, b, t, kh * a.group + r0 + tid - t * a.group, 0)];
+      s_mz[tid] = make_float2(mz.x, mz.y == 0.0f ? 0.0f : 1.0f / mz.y);
     }
     __syncthreads();
     if (j >= fb.keys.lo && j < fb.keys.hi)
@@ -540,181 +446,133 @@ __device__ __forceinline__ float simple_score(const RuleView& rl, float slope, f
   return score_of(r, dot, r.mul) - slope * LOG2E * fabsf(static_cast<float>(pos - j));
 }
 
-template <typename TC>
-__device__ __forceinline__ float dot_row(const float* q, const TC* k, int hd) {
-  float a = 0.0f;
-  for (int d = 0; d < hd; ++d) a = __builtin_fmaf(q[d], static_cast<float>(k[d]), a);
-  return a;
-}
-
-// One work group per (new token, query head): 256 positions at a time, a lane
-// each for the scores, then a lane per output element for the sum over v.
+// The same for prompts, whose scores are formed once more: a lane per position.
 template <typename TC, typename TI>
-__global__ void __launch_bounds__(256) k_paged_attention(PagedView kv, BatchView bt, RuleView rl, TI* __restrict__ out,
-                                                         int64_t out_stride, const TI* __restrict__ q, int64_t q_stride,
-                                                         int n_heads, float2* __restrict__ mz) {
-  __shared__ float s_q[PAGED_MAX_HD], s_p[256], s_red[4];
-  const int h = blockIdx.x, t = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, hd = kv.hd;
-  const SeqRows sr = seq_rows(bt, b);
-  if (t >= sr.n) return;
-  const int row = sr.r0 + t, len = seq_len(bt, kv, b), pos = len - sr.given + t;
-  const int kh = h / (n_heads / kv.n_kv_heads);
-  if (tid < hd) s_q[tid] = static_cast<float>(q[row * q_stride + h * hd + tid]);
-  __syncthreads();
-  float m = MAX_START, z = 0.0f, o = 0.0f;
-  if (pos >= 0) {
-    const RowRule rr = row_rule(rl, b, pos);
-    const float slope = rl.slopes ? rl.slopes[h] : 0.0f;
-    for (int j0 = 0; j0 < len; j0 += 256) {
-      const int j = j0 + tid;
-      float s = -__builtin_inff();
-      if (j < len && seen(rl, rr, b, j)) {
-        const int page = page_of(bt, kv, b, j);
-        if (page >= 0)
-          s = simple_score(rl, slope, dot_row(s_q, reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh), hd), pos, j);
-      }
-      float w = wave_max(s);
-      if ((tid & 63) == 0) s_red[tid >> 6] = w;
-      __syncthreads();
-      w = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-      const float mn = fmaxf(m, w);
-      {
-        const float scale = __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        s_p[tid] = __builtin_amdgcn_exp2f(s - m);
-        __syncthreads();
-        z *= scale;
-        o *= scale;
-        for (int i = 0; i < min(256, len - j0); ++i) {
-          const float p = s_p[i];
-          if (p == 0.0f) continue;
-          z += p;
-          if (tid < hd) {
-            const int page = page_of(bt, kv, b, j0 + i);
-            o = __builtin_fmaf(p, static_cast<float>((reinterpret_cast<const TC*>(kv.v) + elem_of(kv, page, j0 + i, kh))[tid]), o);
-          }
-        }
-      }
-      __syncthreads();
-    }
-  }
-  if (tid < hd) out[row * out_stride + h * hd + tid] = static_cast<TI>(z == 0.0f ? 0.0f : o / z);
-  if (mz && tid == 0) mz[static_cast<int64_t>(row) * n_heads + h] = make_float2(m, z);
-}
-
-// weight of a position: a lane sums its shares over the rows and heads, in order.
-template <typename TC, typename TI>
-__global__ void __launch_bounds__(256) k_paged_weight(PagedView kv, BatchView bt, RuleView rl, const TI* __restrict__ q,
-                                                      int64_t q_stride, int n_heads, const float2* __restrict__ mz) {
+__global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
+  const PagedView& kv = a.kv;
   const int j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, b = blockIdx.z, hd = kv.hd;
-  const int len = seq_len(bt, kv, b), G = n_heads / kv.n_kv_heads;
-  const SeqRows sr = seq_rows(bt, b);
+  const int len = seq_len(a.bt, kv, b);
+  const SeqRows sr = seq_rows(a.bt, b);
   if (j >= len) return;
-  const int page = page_of(bt, kv, b, j);
+  const int page = page_of(a.bt, kv, b, j);
   if (page < 0) return;
   const TC* k = reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh);
   float sum = 0.0f;
   for (int t = 0; t < sr.n; ++t) {
     const int pos = len - sr.given + t;
-    if (pos < 0) continue;
-    const RowRule rr = row_rule(rl, b, pos);
-    if (!seen(rl, rr, b, j)) continue;
-    for (int h = kh * G; h < kh * G + G; ++h) {
-      const int64_t row = sr.r0 + t;
-      float a = 0.0f;
-      for (int d = 0; d < hd; ++d) a = __builtin_fmaf(static_cast<float>(q[row * q_stride + h * hd + d]), static_cast<float>(k[d]), a);
-      const float2 r = mz[row * n_heads + h];
-      if (r.y != 0.0f) sum += __builtin_amdgcn_exp2f(simple_score(rl, rl.slopes ? rl.slopes[h] : 0.0f, a, pos, j) - r.x) / r.y;
+    const RowRule rr = row_rule(a.rl, b, pos);
+    if (!seen(a.rl, rr, b, j)) continue;
+    for (int h = kh * a.group; h < kh * a.group + a.group; ++h) {
+      const TI* q = static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + h * hd;
+      float d = 0.0f;
+      for (int i = 0; i < hd; ++i) d = __builtin_fmaf(static_cast<float>(q[i]), static_cast<float>(k[i]), d);
+      const float2 r = a.part_mz[part_index(a, b, t, h, 0)];
+      if (r.y != 0.0f) sum += __builtin_amdgcn_exp2f(simple_score(a.rl, a.rl.slopes ? a.rl.slopes[h] : 0.0f, d, pos, j) - r.x) / r.y;
     }
   }
   *weight_of(kv, page, j, kh) += sum;
 }
 
-
-struct FewPlan {
-  int n_blocks, chunk, n_splits, score_len;
+// How a call is cut into work groups.  Up to FEW_MOST rows of a sequence and kv
+// head take the 16-row kernel, more the prompt kernel.
+struct Plan {
+  bool few;
+  int block_rows, n_blocks, chunk, n_splits, score_len;
   size_t o_bytes, mz_bytes, score_bytes;
+  size_t bytes() const { return o_bytes + mz_bytes + score_bytes; }
 };
 
-FewPlan few_plan(const PagedView& kv, const BatchView& bt, int n_heads, int window, bool prefix, int n_cu) {
-  FewPlan p{};
+Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu) {
+  Plan p{};
   const int group = n_heads / kv.n_kv_heads;
-  p.n_blocks = (bt.max_new * group + FEW_ROWS - 1) / FEW_ROWS;
+  const int64_t rows = static_cast<int64_t>(bt.max_new) * group;
+  p.few = rows <= FEW_MOST;
+  p.block_rows = p.few ? FEW_ROWS : prompt_block_rows();
+  p.n_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   const int64_t table = static_cast<int64_t>(bt.max_pages) << kv.page_shift;
   int64_t span = std::min<int64_t>(bt.max_len, table);
   p.score_len = static_cast<int>((span + 31) / 32 * 32);
-  // rows of a block are at most FEW_ROWS positions apart, lo goes down to a multiple of 32
-  if (window > 0 && !prefix) span = std::min<int64_t>(span, static_cast<int64_t>(window) + FEW_ROWS + 32);
+  // rows of a block are at most block_rows positions apart, lo goes down to a multiple of 32
+  if (rl.window > 0 && !rl.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(rl.window) + p.block_rows + 32);
   span = std::max<int64_t>(span, 1);
   const int64_t blocks = static_cast<int64_t>(bt.n_seq) * kv.n_kv_heads * p.n_blocks;
-  const int64_t chunk = (span * blocks / (FEW_TARGET * n_cu) + FEW_ROUND) / FEW_ROUND * FEW_ROUND;
-  p.chunk = static_cast<int>(std::min<int64_t>(std::max<int64_t>(chunk, FEW_MIN_CHUNK), FEW_MAX_CHUNK));
+  if (p.few) {
+    const int64_t chunk = (span * blocks / (FEW_TARGET * n_cu) + FEW_ROUND) / FEW_ROUND * FEW_ROUND;
+    p.chunk = static_cast<int>(std::min<int64_t>(std::max<int64_t>(chunk, FEW_MIN_CHUNK), FEW_MAX_CHUNK));
+  } else {
+    const int64_t want = std::max<int64_t>(1, PROMPT_TARGET * n_cu / blocks);
+    p.chunk = static_cast<int>((std::max<int64_t>((span + want - 1) / want, PROMPT_MIN_CHUNK) + 63) / 64 * 64);
+  }
   p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
   const size_t parts = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.n_splits;
   if (p.n_splits > 1) p.o_bytes = parts * kv.hd * sizeof(float);
   if (p.n_splits > 1 || kv.weight) p.mz_bytes = (parts * sizeof(float2) + 15) / 16 * 16;
-  if (kv.weight) p.score_bytes = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.score_len * sizeof(float);
+  if (kv.weight && p.few) p.score_bytes = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.score_len * sizeof(float);
   return p;
 }
 
 template <typename TC, typename TI, int DP>
-hipError_t few(const FewArgs& a, const FewPlan& p, hipStream_t s) {
-  const PagedView& kv = a.kv;
-  const size_t lds = (static_cast<size_t>(p.chunk >> kv.page_shift) + 2) * sizeof(int64_t);
-  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(p.n_splits * kv.n_kv_heads * p.n_blocks, a.bt.n_seq), dim3(256), lds, s, a);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  if (p.n_splits > 1) {
-    hipLaunchKernelGGL((k_attention_join<TI, DP>), dim3(a.bt.max_new * a.n_heads, a.bt.n_seq), dim3(256), 0, s, a);
-    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-  }
-  if (a.scores) {
-    hipLaunchKernelGGL(k_attention_weight, dim3((p.score_len + 255) / 256, kv.n_kv_heads, a.bt.n_seq), dim3(256), 0, s, a);
-    return hipGetLastError();
-  }
-  return hipSuccess;
+hipError_t few(const PagedCall& a, hipStream_t s) {
+  const size_t lds = (static_cast<size_t>(a.chunk >> a.kv.page_shift) + 2) * sizeof(int64_t);
+  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(a.n_splits * a.kv.n_kv_heads * a.n_blocks, a.bt.n_seq), dim3(256), lds, s, a);
+  return hipGetLastError();
+}
+template <typename TC, typename TI>
+hipError_t few(const PagedCall& a, hipStream_t s) {
+  return a.kv.hd <= 64 ? few<TC, TI, 64>(a, s) : a.kv.hd <= 128 ? few<TC, TI, 128>(a, s) : few<TC, TI, 256>(a, s);
+}
+hipError_t launch_attention_few(const PagedCall& a, int kv_type, int io_type, hipStream_t s) {
+  const bool f32 = io_type == MCPM_TYPE_F32;
+  if (kv_type == MCPM_TYPE_F32) return few<float, float>(a, s);
+  if (kv_type == MCPM_TYPE_F16) return f32 ? few<_Float16, float>(a, s) : few<_Float16, _Float16>(a, s);
+  return f32 ? few<__bf16, float>(a, s) : few<__bf16, __bf16>(a, s);
+}
+
+template <typename TI>
+hipError_t join(const PagedCall& a, hipStream_t s) {
+  const dim3 grid(a.bt.max_new * a.n_heads, a.bt.n_seq);
+  if (a.kv.hd <= 64) hipLaunchKernelGGL((k_attention_join<TI, 64>), grid, dim3(256), 0, s, a);
+  else if (a.kv.hd <= 128) hipLaunchKernelGGL((k_attention_join<TI, 128>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_attention_join<TI, 256>), grid, dim3(256), 0, s, a);
+  return hipGetLastError();
 }
 
 template <typename TC, typename TI>
-hipError_t attention(const PagedView& kv, const BatchView& bt, const RuleView& rl, void* out, int64_t out_stride,
-                     const void* q, int64_t q_stride, int n_heads, char* scratch, int n_cu, hipStream_t s) {
-  const int group = n_heads / kv.n_kv_heads;
-  if (static_cast<int64_t>(bt.max_new) * group <= FEW_MOST) {
-    const FewPlan p = few_plan(kv, bt, n_heads, rl.window, rl.prefix != nullptr, n_cu);
-    FewArgs a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.n_blocks, p.chunk, p.n_splits,
-              reinterpret_cast<float*>(scratch), p.mz_bytes ? reinterpret_cast<float2*>(scratch + p.o_bytes) : nullptr,
-              p.score_bytes ? reinterpret_cast<float*>(scratch + p.o_bytes + p.mz_bytes) : nullptr, p.score_len, bt.max_new * group};
-    return kv.hd <= 64 ? few<TC, TI, 64>(a, p, s) : kv.hd <= 128 ? few<TC, TI, 128>(a, p, s) : few<TC, TI, 256>(a, p, s);
-  }
-  float2* mz = kv.weight ? reinterpret_cast<float2*>(scratch) : nullptr;
-  hipLaunchKernelGGL((k_paged_attention<TC, TI>), dim3(n_heads, bt.max_new, bt.n_seq), dim3(256), 0, s, kv, bt, rl,
-                     static_cast<TI*>(out), out_stride, static_cast<const TI*>(q), q_stride, n_heads, mz);
-  if (hipError_t e = hipGetLastError(); e != hipSuccess || !mz) return e;
-  hipLaunchKernelGGL((k_paged_weight<TC, TI>), dim3((bt.max_len + 255) / 256, kv.n_kv_heads, bt.n_seq), dim3(256), 0, s,
-                     kv, bt, rl, static_cast<const TI*>(q), q_stride, n_heads, mz);
+hipError_t prompt_weight(const PagedCall& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_prompt_weight<TC, TI>), dim3((a.score_len + 255) / 256, a.kv.n_kv_heads, a.bt.n_seq), dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
 }  // namespace
 
 size_t paged_attention_scratch(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu) {
-  if (static_cast<int64_t>(bt.max_new) * (n_heads / kv.n_kv_heads) <= FEW_MOST) {
-    const FewPlan p = few_plan(kv, bt, n_heads, rl.window, rl.prefix != nullptr, n_cu);
-    return p.o_bytes + p.mz_bytes + p.score_bytes;
-  }
-  return kv.weight ? static_cast<size_t>(bt.n_rows) * n_heads * sizeof(float2) : 0;
+  return plan_of(kv, bt, rl, n_heads, n_cu).bytes();
 }
 
 hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type,
                                   void* out, int64_t out_stride, const void* q, int64_t q_stride, int n_heads,
                                   void* scratch, int n_cu, hipStream_t s) {
-  const bool f32 = io_type == MCPM_TYPE_F32;
+  const Plan p = plan_of(kv, bt, rl, n_heads, n_cu);
+  const int group = n_heads / kv.n_kv_heads;
   char* sc = static_cast<char*>(scratch);
-  if (kv_type == MCPM_TYPE_F32) return attention<float, float>(kv, bt, rl, out, out_stride, q, q_stride, n_heads, sc, n_cu, s);
-  if (kv_type == MCPM_TYPE_F16)
-    return f32 ? attention<_Float16, float>(kv, bt, rl, out, out_stride, q, q_stride, n_heads, sc, n_cu, s)
-               : attention<_Float16, _Float16>(kv, bt, rl, out, out_stride, q, q_stride, n_heads, sc, n_cu, s);
-  return f32 ? attention<__bf16, float>(kv, bt, rl, out, out_stride, q, q_stride, n_heads, sc, n_cu, s)
-             : attention<__bf16, __bf16>(kv, bt, rl, out, out_stride, q, q_stride, n_heads, sc, n_cu, s);
+  const PagedCall a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.block_rows, p.n_blocks, p.chunk, p.n_splits,
+                    reinterpret_cast<float*>(sc), p.mz_bytes ? reinterpret_cast<float2*>(sc + p.o_bytes) : nullptr,
+                    p.score_bytes ? reinterpret_cast<float*>(sc + p.o_bytes + p.mz_bytes) : nullptr, p.score_len, bt.max_new * group};
+  hipError_t e = p.few ? launch_attention_few(a, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
+  if (e != hipSuccess) return e;
+  if (p.n_splits > 1) {
+    e = io_type == MCPM_TYPE_F32 ? join<float>(a, s) : io_type == MCPM_TYPE_F16 ? join<_Float16>(a, s) : join<__bf16>(a, s);
+    if (e != hipSuccess) return e;
+  }
+  if (!kv.weight || !p.score_len) return hipSuccess;
+  if (p.few) {
+    hipLaunchKernelGGL(k_attention_weight, dim3((p.score_len + 255) / 256, kv.n_kv_heads, bt.n_seq), dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  const bool f32 = io_type == MCPM_TYPE_F32;
+  if (kv_type == MCPM_TYPE_F32) return prompt_weight<float, float>(a, s);
+  if (kv_type == MCPM_TYPE_F16) return f32 ? prompt_weight<_Float16, float>(a, s) : prompt_weight<_Float16, _Float16>(a, s);
+  return f32 ? prompt_weight<__bf16, float>(a, s) : prompt_weight<__bf16, __bf16>(a, s);
 }
 
 }  // namespace mcpm

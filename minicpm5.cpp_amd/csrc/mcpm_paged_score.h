@@ -120,4 +120,108 @@ __device__ __forceinline__ KeyRange key_range(const RuleView& rl, int b, int pos
   return KeyRange{lo & ~31, hi};
 }
 
+// A call as its kernels see it.  A row block is `block_rows` rows of a sequence
+// (new tokens x the kv head's query heads, token by token); its positions are cut
+// into chunks of `chunk`, a work group each.
+struct PagedCall {
+  PagedView kv;
+  BatchView bt;
+  RuleView rl;
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;
+  int n_heads, group, block_rows, n_blocks;  // query heads per kv head; row blocks per (sequence, kv head)
+  int chunk, n_splits;
+  float* part_o;    // [seq][new token][head][split][hd], unnormalised
+  float2* part_mz;  // [seq][new token][head][split]; with weights, the first is the row's own at the end
+  float* scores;    // [seq][kv head][row of the sequence][score_len], or null
+  int score_len, score_rows;
+};
+
+__device__ __forceinline__ int64_t part_index(const PagedCall& a, int b, int t, int head, int split) {
+  return ((static_cast<int64_t>(b) * a.bt.max_new + t) * a.n_heads + head) * a.n_splits + split;
+}
+
+// The positions of a row block.
+struct RowBlock {
+  int r_end;  // rows of the sequence
+  int pos0;   // position of the sequence's first new token
+  int first, last;  // positions of the block's first and last row
+  KeyRange keys;
+};
+__device__ __forceinline__ RowBlock row_block(const PagedCall& a, int b, int rb, const SeqRows& sr, int len) {
+  const int pos0 = len - sr.given, r_end = sr.n * a.group;
+  const int first = pos0 + rb * a.block_rows / a.group;
+  const int last = pos0 + (min(rb * a.block_rows + a.block_rows, r_end) - 1) / a.group;
+  return RowBlock{r_end, pos0, first, last, key_range(a.rl, b, first, last, len)};
+}
+
+// Page offsets of a chunk (a page outside the pool stands at the first one, to be masked);
+// whether all of this lane's are in the pool.
+__device__ __forceinline__ bool load_page_offsets(const BatchView& bt, const PagedView& kv, int b, int c0, int c1, int64_t* s_off) {
+  bool ok = true;
+  const int first = c0 >> kv.page_shift, n = ((c1 - 1) >> kv.page_shift) - first + 1;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const int page = page_of(bt, kv, b, (first + i) << kv.page_shift);
+    s_off[i] = page < 0 ? 0 : page * kv.page_stride;
+    ok = ok && page >= 0;
+  }
+  return ok;
+}
+
+// The plain computation of one row over positions [c0, c1), by the whole work
+// group, for values that the matrix products cannot keep apart: a share of 0
+// times what a masked place holds.  Returns this lane's element tid of sum
+// p v, and (m, z).
+template <typename TC, typename TI>
+__device__ __forceinline__ float exact_row(const PagedCall& a, int b, int kh, int row, int head, int pos, int c0, int c1, float* s_q,
+                                        float* s_p, float* s_red, float2* mz) {
+  const PagedView& kv = a.kv;
+  const int tid = threadIdx.x, hd = kv.hd;
+  __syncthreads();
+  if (tid < hd) s_q[tid] = static_cast<float>(static_cast<const TI*>(a.q)[row * a.q_stride + head * hd + tid]);
+  __syncthreads();
+  const ScoreRule sr = score_rule(a.rl);
+  const RowRule rr = row_rule(a.rl, b, pos);
+  const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
+  float m = MAX_START, z = 0.0f, o = 0.0f;
+  for (int j0 = c0; j0 < c1; j0 += 256) {
+    const int j = j0 + tid;
+    float s = -__builtin_inff();
+    const int page = j < c1 && pos >= 0 && seen(a.rl, rr, b, j) ? page_of(a.bt, kv, b, j) : -1;
+    if (page >= 0) {
+      const TC* k = reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh);
+      float d = 0.0f;
+      for (int i = 0; i < hd; ++i) d = __builtin_fmaf(s_q[i], static_cast<float>(k[i]), d);
+      s = score_of(sr, d, sr.mul) - slope * fabsf(static_cast<float>(pos - j));
+    }
+    float w = wave_max(s);
+    if ((tid & 63) == 0) s_red[tid >> 6] = w;
+    __syncthreads();
+    w = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    const float mn = fmaxf(m, w), scale = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    s_p[tid] = __builtin_amdgcn_exp2f(s - m);
+    __syncthreads();
+    z *= scale;
+    o *= scale;
+    for (int i = 0; i < min(256, c1 - j0); ++i) {
+      const float p = s_p[i];
+      if (p == 0.0f) continue;
+      z += p;
+      if (tid < hd) {
+        const int pg = page_of(a.bt, kv, b, j0 + i);  // p != 0: in the pool
+        if (pg >= 0) o = __builtin_fmaf(p, static_cast<float>((reinterpret_cast<const TC*>(kv.v) + elem_of(kv, pg, j0 + i, kh))[tid]), o);
+      }
+    }
+    __syncthreads();
+  }
+  *mz = make_float2(m, z);
+  return o;
+}
+
+// The prompt kernels (mcpm_paged_prompt.hip): row blocks of prompt_block_rows rows.
+int prompt_block_rows();
+hipError_t launch_attention_prompt(const PagedCall& a, int kv_type, int io_type, hipStream_t s);
+
 }  // namespace mcpm
