@@ -207,7 +207,7 @@ int mcpm_op_time(mcpm_ctx *ctx, double *total_ms, int64_t *launches);
  * pos_stride and head_stride less than 2^31.
  * A contiguous cache [max_seq_len][n_kv_heads][head_dim] is such a pool, its
  * pages in order.  `weight` (may be NULL): float [n_pages][n_kv_heads][page_size],
- * the attention each cached position has received. */
+ * 16-byte aligned, the attention each cached position has received. */
 typedef struct {
     int type;
     int n_pages, page_size;

@@ -84,9 +84,11 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
                                   void* out, int64_t out_stride, const void* q, int64_t q_stride, int n_heads,
                                   void* scratch, int n_cu, hipStream_t s);
 
+// Bytes of scratch that launch_paged_evict needs.
+size_t paged_evict_scratch(const PagedView& kv, const BatchView& bt, int first, int recent);
 hipError_t launch_paged_evict(const PagedView& kv, int kv_type, const BatchView& bt, int budget, int first, int recent,
-                              const int* dst_pages, int max_dst_pages, int* kept, int* dst_lens, hipStream_t s);
+                              const int* dst_pages, int max_dst_pages, int* kept, int* dst_lens, void* scratch, hipStream_t s);
 
-hipError_t launch_process_logits(float* logits, const mcpm_logit_rules& r, hipStream_t s);
+hipError_t launch_process_logits(float* logits, const mcpm_logit_rules& r, int n_cu, hipStream_t s);
 
 }  // namespace mcpm

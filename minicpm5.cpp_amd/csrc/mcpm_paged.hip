@@ -1,5 +1,8 @@
 // mcpm_paged.hip -- writing side of the paged cache: the append of new tokens
 // (with the rotation of k and q) and the eviction by accumulated weight.
+#include <climits>
+#include <cmath>
+
 #include "mcpm_device.h"
 #include "mcpm_paged.h"
 
@@ -107,78 +110,315 @@ __device__ __forceinline__ unsigned weight_key(float w) {
 
 constexpr int EV_T = 1024;
 
-// One work group per (sequence, kv head): the key of the smallest kept weight
-// by four 8-bit histogram passes, then the kept positions in order.
-__global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView bt, int budget, int first, int recent,
-                                                       int* __restrict__ kept, int* __restrict__ dst_lens) {
-  __shared__ unsigned hist[256];
-  __shared__ unsigned s_key, s_need;
-  __shared__ int s_wave[2][EV_T / 64];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const int len = seq_len(bt, kv, b);
-  int* out = kept + (static_cast<int64_t>(b) * kv.n_kv_heads + h) * budget;
-  const int n_keep = min(len, budget);
-  if (h == 0 && tid == 0) dst_lens[b] = n_keep;
-  for (int i = n_keep + tid; i < budget; i += EV_T) out[i] = -1;
-  if (len <= budget) {
-    for (int i = tid; i < len; i += EV_T) out[i] = i;
-    return;
-  }
-  const int lo = first, hi = len - recent;  // candidates
-  auto key_at = [&](int j) {
-    const int page = page_of(bt, kv, b, j);
-    return page < 0 ? 0u : weight_key(*weight_of(kv, page, j, h));
-  };
-  if (tid == 0) {
-    s_key = 0;
-    s_need = budget - first - recent;
+// For each of N counts: the sum over the lanes before this one in the work group;
+// `all` gets the sums over every lane.
+template <int N, int WAVES>
+__device__ __forceinline__ void block_prefix(int (&v)[N], int (*s_wave)[WAVES], int (&all)[N]) {
+  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+  int x[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    x[n] = v[n];
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      const int y = __shfl_up(x[n], s);
+      x[n] += lane >= s ? y : 0;
+    }
   }
   __syncthreads();
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += EV_T) hist[i] = 0;
-    __syncthreads();
-    const unsigned pre = s_key, need = s_need;
-    const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
-    for (int j = lo + tid; j < hi; j += EV_T) {
-      const unsigned key = key_at(j);
-      if ((key & mask) == pre) atomicAdd(&hist[(key >> shift) & 255], 1u);
+  if (lane == 63)
+#pragma unroll
+    for (int n = 0; n < N; ++n) s_wave[n][wv] = x[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    int before = 0;
+    all[n] = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+      const int c = s_wave[n][w];
+      before += w < wv ? c : 0;
+      all[n] += c;
     }
-    __syncthreads();
-    if (tid == 0) {
-      unsigned left = need;
-      int d = 255;
-      while (d > 0 && hist[d] < left) left -= hist[d--];
-      s_key = pre | (static_cast<unsigned>(d) << shift);
-      s_need = left;
-    }
-    __syncthreads();
+    v[n] = before + x[n] - v[n];
   }
-  const unsigned edge = s_key, need = s_need;  // kept: key > edge, and the first `need` that equal it
-  int n_eq = 0, n_out = 0;
-  for (int j0 = 0; j0 < len; j0 += EV_T) {
-    const int j = j0 + tid;
-    const bool in = j < len, mid = in && j >= lo && j < hi;
-    const unsigned key = mid ? key_at(j) : 0u;
-    const bool eq = mid && key == edge;
-    const unsigned long long below = (1ull << lane) - 1;
-    const unsigned long long me = __ballot(eq);
-    if (lane == 0) s_wave[0][wv] = __popcll(me);
-    __syncthreads();
-    int rank = n_eq + __popcll(me & below);
-    for (int w = 0; w < EV_T / 64; ++w) {
-      if (w < wv) rank += s_wave[0][w];
-      n_eq += s_wave[0][w];
+}
+
+// The keys of V consecutive positions from j, a multiple of V, on; 0 outside
+// [first, end).  Inside one page wherever pages hold that many: 16-byte loads.
+template <int V>
+__device__ __forceinline__ void load_keys(const PagedView& kv, const BatchView& bt, int b, int h, int j, int end, unsigned (&key)[V]) {
+  if (kv.page_mask >= V - 1) {
+    const int page = j < end ? page_of(bt, kv, b, j) : -1;
+    f32x4 w[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = page >= 0 ? *reinterpret_cast<const f32x4*>(weight_of(kv, page, j, h) + 4 * i) : f32x4{NAN, NAN, NAN, NAN};
+#pragma unroll
+    for (int i = 0; i < V; ++i) key[i] = weight_key(w[i / 4][i % 4]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const int page = j + i < end ? page_of(bt, kv, b, j + i) : -1;
+      key[i] = page >= 0 ? weight_key(*weight_of(kv, page, j + i, h)) : 0u;
     }
-    const bool keep = in && (!mid || key > edge || (eq && rank < static_cast<int>(need)));
-    const unsigned long long mk = __ballot(keep);
-    if (lane == 0) s_wave[1][wv] = __popcll(mk);
-    __syncthreads();
-    int at = n_out + __popcll(mk & below);
-    for (int w = 0; w < EV_T / 64; ++w) {
-      if (w < wv) at += s_wave[1][w];
-      n_out += s_wave[1][w];
+  }
+}
+
+// What is kept whatever it weighs, and the end of the list.  Returns whether there is
+// anything to choose.
+__device__ __forceinline__ bool kept_ends(int len, int budget, int first, int recent, int lane, int lanes, int* out) {
+  for (int i = min(len, budget) + lane; i < budget; i += lanes) out[i] = -1;
+  if (len <= budget) {
+    for (int i = lane; i < len; i += lanes) out[i] = i;
+    return false;
+  }
+  for (int i = lane; i < first; i += lanes) out[i] = i;
+  for (int i = lane; i < recent; i += lanes) out[budget - recent + i] = len - recent + i;
+  return budget - first - recent > 0;
+}
+
+// The bin, from the top, in which the running count reaches `need`: BINS counts
+// in LDS, PER a lane (lane t has the ones that end at BINS - 1 - PER t).
+struct Edge {
+  int bin, need, count;  // the bin, how many of its values are needed, how many it has
+};
+template <int PER, int WAVES>
+__device__ __forceinline__ void find_edge(const int* hist, int bins, int need, int (*s_wave)[WAVES], Edge* s_edge) {
+  const int top = bins - 1 - PER * static_cast<int>(threadIdx.x);
+  int c[PER], sum[1] = {0}, total[1];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    c[i] = hist[top - i];
+    sum[0] += c[i];
+  }
+  const int mine = sum[0];
+  block_prefix(sum, s_wave, total);
+  int above = sum[0];
+  if (above < need && above + mine >= need) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if (above < need && above + c[i] >= need) *s_edge = Edge{top - i, need - above, c[i]};
+      above += c[i];
     }
-    if (keep && at < n_keep) out[at] = j;
+  }
+  __syncthreads();
+}
+
+// Up to 16 x 1024 candidates: one work group per (sequence, kv head).  A lane has
+// V consecutive positions, whose keys stay in registers.  The key of the smallest weight
+// kept comes from histograms of 11, 11 and 10 bits: the first one has the weight's
+// exponent and two bits of its fraction, so that lanes seldom meet in a bin, the
+// others count only what is left.  Kept then are the larger keys and, of those
+// equal to it, the first ones.
+constexpr int EV_BINS = 2048;
+
+template <int V>
+__global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView bt, int budget, int first, int recent,
+                                                       int* __restrict__ kept, int* __restrict__ dst_lens) {
+  __shared__ int hist[EV_BINS];
+  __shared__ int s_wave[1][EV_T / 64];
+  __shared__ Edge s_edge;
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int len = seq_len(bt, kv, b);
+  int* out = kept + (static_cast<int64_t>(b) * kv.n_kv_heads + h) * budget;
+  if (h == 0 && tid == 0) dst_lens[b] = min(len, budget);
+  if (!kept_ends(len, budget, first, recent, tid, EV_T, out)) return;
+  const int begin = first & ~(V - 1), end = len - recent;  // candidates are [first, end)
+  const int j0 = begin + tid * V;
+  unsigned key[V];
+  load_keys<V>(kv, bt, b, h, j0, end, key);
+  auto candidate = [&](int i) { return j0 + i >= first && j0 + i < end; };
+  unsigned edge = 0;
+  int need = budget - first - recent;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : EV_BINS;
+    const unsigned mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
+    for (int i = tid; i < EV_BINS; i += EV_T) hist[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (candidate(i) && (key[i] & mask) == edge) atomicAdd(&hist[(key[i] >> shift) & (bins - 1)], 1);
+    __syncthreads();
+    find_edge<EV_BINS / EV_T>(hist, EV_BINS, need, s_wave, &s_edge);
+    edge |= static_cast<unsigned>(s_edge.bin) << shift;
+    need = s_edge.need;
+  }
+  unsigned keep = 0;  // bit i: position i of the lane's is kept
+  int n[1] = {0}, all[1];
+  if (s_edge.count != need) {  // the first `need` of the equal ones
+#pragma unroll
+    for (int i = 0; i < V; ++i) n[0] += candidate(i) && key[i] == edge;
+    block_prefix(n, s_wave, all);
+  } else {
+    need = INT_MAX;
+  }
+  int rank = n[0];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (candidate(i) && (key[i] > edge || (key[i] == edge && rank++ < need))) keep |= 1u << i;
+  n[0] = __popc(keep);
+  block_prefix(n, s_wave, all);
+  int o = first + n[0];
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (keep >> i & 1) out[o++] = j0 + i;
+}
+
+// More candidates: the same over slices of SL_T x SL_V positions, a work group
+// each, in three launches, for one CU has neither the registers nor the issue
+// slots for a long cache (65,536 candidates of one head in one work group: 84 us).
+//   count   each slice's histogram of the top 11 bits
+//   edge    the bin of the smallest kept key, from all slices' histograms; the
+//           candidates in it go into one list, in any order
+//   write   the exact edge from the list (every slice for itself), and the kept
+//           positions at the place that the counts of the slices before give
+constexpr int SL_T = 256, SL_V = 16, SL_N = SL_T * SL_V;
+
+struct EvictLong {
+  uint16_t* hist;  // [pair][slice][EV_BINS]
+  int* before;     // [pair][slice]: kept in earlier slices by the first 11 bits alone
+  int* n_list;     // [pair]
+  int* need;       // [pair]: how many of the list are kept
+  uint2* list;     // [pair][slices * SL_N]: (key, position)
+  int slices;
+};
+
+template <int STEP>
+__global__ void __launch_bounds__(SL_T) k_evict_long(PagedView kv, BatchView bt, int budget, int first, int recent, const EvictLong g,
+                                                     int* __restrict__ kept, int* __restrict__ dst_lens) {
+  __shared__ int hist[EV_BINS];
+  __shared__ int s_wave[1][SL_T / 64];
+  __shared__ Edge s_edge;
+  __shared__ int s_sum[3];
+  const int slice = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int64_t pair = static_cast<int64_t>(b) * kv.n_kv_heads + h;
+  const int len = seq_len(bt, kv, b);
+  int* out = kept + pair * budget;
+  if constexpr (STEP == 0) {
+    if (slice == 0 && tid == 0) g.n_list[pair] = 0;
+    if (slice == 0 && h == 0 && tid == 0) dst_lens[b] = min(len, budget);
+    kept_ends(len, budget, first, recent, slice * SL_T + tid, g.slices * SL_T, out);
+  }
+  if (len <= budget || budget - first - recent == 0) return;
+  const int begin = first & ~(SL_V - 1), end = len - recent;
+  const int n_slices = (end - begin + SL_N - 1) / SL_N;
+  if (slice >= n_slices) return;
+  const int j0 = begin + slice * SL_N + tid * SL_V;
+  unsigned key[SL_V];
+  load_keys<SL_V>(kv, bt, b, h, j0, end, key);
+  auto candidate = [&](int i) { return j0 + i >= first && j0 + i < end; };
+  auto clear = [&] {
+    for (int i = tid; i < EV_BINS; i += SL_T) hist[i] = 0;
+    if (tid < 3) s_sum[tid] = 0;
+    __syncthreads();
+  };
+  constexpr int PER = EV_BINS / SL_T;
+  uint16_t* mine = g.hist + (pair * g.slices + slice) * EV_BINS;
+  uint2* list = g.list + pair * g.slices * SL_N;
+  if constexpr (STEP == 0) {
+    clear();
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i)
+      if (candidate(i)) atomicAdd(&hist[key[i] >> 21], 1);
+    __syncthreads();
+    uint32_t w[PER / 2];
+#pragma unroll
+    for (int i = 0; i < PER / 2; ++i) w[i] = static_cast<uint32_t>(hist[tid * PER + 2 * i]) | static_cast<uint32_t>(hist[tid * PER + 2 * i + 1]) << 16;
+    *reinterpret_cast<u32x4*>(mine + tid * PER) = u32x4{w[0], w[1], w[2], w[3]};
+  } else if constexpr (STEP == 1) {
+    clear();
+    int sum[PER] = {}, before[PER] = {};  // of all slices, and of those before this one
+    const uint16_t* other = g.hist + pair * g.slices * EV_BINS + tid * PER;
+#pragma unroll 4
+    for (int s = 0; s < n_slices; ++s) {
+      const u32x4 w = *reinterpret_cast<const u32x4*>(other + static_cast<int64_t>(s) * EV_BINS);
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int c = w[i / 2] >> (16 * (i % 2)) & 0xffff;
+        sum[i] += c;
+        before[i] += s < slice ? c : 0;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) hist[tid * PER + i] = sum[i];
+    __syncthreads();
+    find_edge<PER>(hist, EV_BINS, budget - first - recent, s_wave, &s_edge);
+    const unsigned bin = s_edge.bin;
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) above += tid * PER + i > static_cast<int>(bin) ? before[i] : 0;
+    int n[1] = {above}, all[1];
+    block_prefix(n, s_wave, all);
+    if (tid == 0) g.before[pair * g.slices + slice] = all[0];
+    if (tid == 0 && slice == 0) g.need[pair] = s_edge.need;
+    n[0] = 0;
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i) n[0] += candidate(i) && key[i] >> 21 == bin;
+    block_prefix(n, s_wave, all);
+    if (tid == 0) s_sum[0] = all[0] ? atomicAdd(&g.n_list[pair], all[0]) : 0;
+    __syncthreads();
+    int o = s_sum[0] + n[0];
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i)
+      if (candidate(i) && key[i] >> 21 == bin) list[o++] = make_uint2(key[i], j0 + i);
+  } else {
+    // The list, in registers as far as OWN entries a lane go.
+    constexpr int OWN = 16;
+    const int n_list = g.n_list[pair];
+    int need = g.need[pair];
+    uint2 own[OWN];
+#pragma unroll
+    for (int k = 0; k < OWN; ++k) own[k] = list[min(tid + k * SL_T, n_list - 1)];
+    auto members = [&](const auto& f) {
+#pragma unroll
+      for (int k = 0; k < OWN; ++k)
+        if (tid + k * SL_T < n_list) f(own[k]);
+      for (int i = tid + OWN * SL_T; i < n_list; i += SL_T) f(list[i]);
+    };
+    unsigned edge = list[0].x & ~0u << 21;
+#pragma unroll 1
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : EV_BINS;
+      const unsigned mask = pass == 1 ? ~0u << 21 : ~0u << 10;
+      clear();
+      members([&](const uint2& x) {
+        if ((x.x & mask) == edge) atomicAdd(&hist[(x.x >> shift) & (bins - 1)], 1);
+      });
+      __syncthreads();
+      find_edge<PER>(hist, EV_BINS, need, s_wave, &s_edge);
+      edge |= static_cast<unsigned>(s_edge.bin) << shift;
+      need = s_edge.need;
+    }
+    // members of earlier slices: larger ones, equal ones
+    int c[2] = {0, 0};
+    const int slice_begin = begin + slice * SL_N;
+    members([&](const uint2& x) {
+      if (static_cast<int>(x.y) < slice_begin) {
+        c[0] += x.x > edge;
+        c[1] += x.x == edge;
+      }
+    });
+    if (c[0]) atomicAdd(&s_sum[0], c[0]);
+    if (c[1]) atomicAdd(&s_sum[1], c[1]);
+    __syncthreads();
+    const int larger = s_sum[0], equal = s_sum[1];
+    int n[1] = {0}, all[1];
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i) n[0] += candidate(i) && key[i] == edge;
+    block_prefix(n, s_wave, all);
+    int rank = equal + n[0];
+    unsigned keep = 0;
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i)
+      if (candidate(i) && (key[i] > edge || (key[i] == edge && rank++ < need))) keep |= 1u << i;
+    n[0] = __popc(keep);
+    block_prefix(n, s_wave, all);
+    int o = first + g.before[pair * g.slices + slice] + larger + min(equal, need) + n[0];
+#pragma unroll
+    for (int i = 0; i < SL_V; ++i)
+      if (keep >> i & 1) out[o++] = j0 + i;
   }
 }
 
@@ -230,11 +470,45 @@ hipError_t launch_paged_append(const PagedView& kv, int kv_type, const BatchView
   return hipGetLastError();
 }
 
+namespace {
+constexpr int EV_MOST = 16 * EV_T;
+// Positions from the first candidate's run of SL_V on, at most.
+int evict_span(const BatchView& bt, int first, int recent) { return bt.max_len - recent - (first & ~(SL_V - 1)); }
+}  // namespace
+
+size_t paged_evict_scratch(const PagedView& kv, const BatchView& bt, int first, int recent) {
+  const int n = evict_span(bt, first, recent);
+  if (n <= EV_MOST) return 0;
+  const size_t pairs = static_cast<size_t>(bt.n_seq) * kv.n_kv_heads, slices = (static_cast<size_t>(n) + SL_N - 1) / SL_N;
+  return pairs * slices * (EV_BINS * sizeof(uint16_t) + SL_N * sizeof(uint2) + sizeof(int)) + 2 * pairs * sizeof(int);
+}
+
 hipError_t launch_paged_evict(const PagedView& kv, int kv_type, const BatchView& bt, int budget, int first, int recent,
-                              const int* dst_pages, int max_dst_pages, int* kept, int* dst_lens, hipStream_t s) {
+                              const int* dst_pages, int max_dst_pages, int* kept, int* dst_lens, void* scratch, hipStream_t s) {
   const int esz = kv_type == MCPM_TYPE_F32 ? 4 : 2;
-  hipLaunchKernelGGL(k_evict_select, dim3(kv.n_kv_heads, bt.n_seq), dim3(EV_T), 0, s, kv, bt, budget, first, recent, kept,
-                     dst_lens);
+  const dim3 grid(kv.n_kv_heads, bt.n_seq);
+  const int n = evict_span(bt, first, recent);
+  if (n <= 4 * EV_T) {
+    hipLaunchKernelGGL(k_evict_select<4>, grid, dim3(EV_T), 0, s, kv, bt, budget, first, recent, kept, dst_lens);
+  } else if (n <= EV_MOST) {
+    hipLaunchKernelGGL(k_evict_select<16>, grid, dim3(EV_T), 0, s, kv, bt, budget, first, recent, kept, dst_lens);
+  } else {
+    const int64_t pairs = static_cast<int64_t>(bt.n_seq) * kv.n_kv_heads;
+    EvictLong g{};
+    g.slices = (n + SL_N - 1) / SL_N;
+    char* p = static_cast<char*>(scratch);
+    g.hist = reinterpret_cast<uint16_t*>(p);
+    p += pairs * g.slices * EV_BINS * sizeof(uint16_t);
+    g.list = reinterpret_cast<uint2*>(p);
+    p += pairs * g.slices * SL_N * sizeof(uint2);
+    g.before = reinterpret_cast<int*>(p);
+    g.n_list = g.before + pairs * g.slices;
+    g.need = g.n_list + pairs;
+    const dim3 slices(g.slices, kv.n_kv_heads, bt.n_seq);
+    hipLaunchKernelGGL(k_evict_long<0>, slices, dim3(SL_T), 0, s, kv, bt, budget, first, recent, g, kept, dst_lens);
+    hipLaunchKernelGGL(k_evict_long<1>, slices, dim3(SL_T), 0, s, kv, bt, budget, first, recent, g, kept, dst_lens);
+    hipLaunchKernelGGL(k_evict_long<2>, slices, dim3(SL_T), 0, s, kv, bt, budget, first, recent, g, kept, dst_lens);
+  }
   if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   const int64_t lanes = static_cast<int64_t>(budget) * (2 * (kv.hd * esz / 16));
   hipLaunchKernelGGL(k_evict_copy, dim3(static_cast<unsigned>((lanes + 255) / 256), kv.n_kv_heads, bt.n_seq), dim3(256), 0, s, kv, bt,

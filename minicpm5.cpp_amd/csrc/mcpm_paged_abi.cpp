@@ -45,6 +45,7 @@ int view_kv(const mcpm_paged_kv* kv, const char* fn, PagedView& out) {
     if (st < kv->head_dim || st % step) return fail(MCPM_ERR_ARG, std::string(fn) + ": strides must be multiples of 16 bytes, at least head_dim");
   if (kv->pos_stride > INT32_MAX || kv->head_stride > INT32_MAX)
     return fail(MCPM_ERR_ARG, std::string(fn) + ": pos_stride and head_stride must be less than 2^31");
+  if (!aligned16(kv->weight)) return fail(MCPM_ERR_ARG, std::string(fn) + ": weight must be 16-byte aligned");
   int shift = 0;
   while ((1 << shift) < kv->page_size) ++shift;
   out = PagedView{static_cast<char*>(kv->k), static_cast<char*>(kv->v), kv->weight, kv->page_stride, kv->pos_stride,
@@ -173,7 +174,9 @@ int mcpm_paged_evict(mcpm_ctx* c, const mcpm_paged_kv* kv, const mcpm_paged_batc
   if (!bt.n_seq) return MCPM_OK;
   DeviceScope dev(c->device);
   MCPM_HIP(dev.status());
-  MCPM_HIP(launch_paged_evict(kvv, kv->type, bt, budget, first, recent, dst_pages, max_dst_pages, kept, dst_lens, c->stream));
+  rc = ensure_paged_scratch(c, paged_evict_scratch(kvv, bt, first, recent));
+  if (rc) return rc;
+  MCPM_HIP(launch_paged_evict(kvv, kv->type, bt, budget, first, recent, dst_pages, max_dst_pages, kept, dst_lens, c->d_paged, c->stream));
   return MCPM_OK;
 }
 
@@ -191,7 +194,7 @@ int mcpm_process_logits(mcpm_ctx* c, float* logits, const mcpm_logit_rules* r) {
   if (!r->n_seq) return MCPM_OK;
   DeviceScope dev(c->device);
   MCPM_HIP(dev.status());
-  MCPM_HIP(launch_process_logits(logits, *r, c->stream));
+  MCPM_HIP(launch_process_logits(logits, *r, c->n_cu, c->stream));
   return MCPM_OK;
 }
 

@@ -578,7 +578,7 @@ def test_evict_budgets(ctx, budget, first, recent):
     check_evict(ctx, "budget", F16, 3, 40, 8, [300, 65, 64, 0], budget, first, recent, heavy, order="hpd", pad=1)
 
 
-@pytest.mark.parametrize("n", [1023, 1024, 1025, 2049, 5000, 20001])
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 2049, 4300, 5000, 16500, 20001, 65700, 131500])
 def test_evict_lengths(ctx, n):
     check_evict(ctx, "length", F16, 1, 8, 64, [n], n // 3, 4, 100, ties)
     check_evict(ctx, "length", F16, 1, 8, 64, [n], n // 3, 4, 100, heavy)

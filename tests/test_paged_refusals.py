@@ -143,6 +143,8 @@ def test_evictions(lib):
     refused(lib, evict(lib, budget=17), mcpm.ERR_ARG, "less than budget")
     refused(lib, evict(lib, max_dst=0), mcpm.ERR_ARG, "less than budget")
     refused(lib, evict(lib, kv_=kv()), mcpm.ERR_ARG, "null weight")
+    refused(lib, evict(lib, kv_=kv(weight=A + 4)), mcpm.ERR_ARG, "weight must be 16-byte aligned")
+    refused(lib, attention(lib, kv_=kv(weight=A + 8)), mcpm.ERR_ARG, "weight must be 16-byte aligned")
     for over in (dict(dst=None), dict(kept=None), dict(lens=None)):
         refused(lib, evict(lib, **over), mcpm.ERR_ARG, "null weight, dst_pages")
     refused(lib, evict(lib, dst=A), mcpm.ERR_ARG, "memory of their own")
