@@ -243,7 +243,10 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   FewTile<TC, TI, DP> tile;
   tile.load_q(row_in && pos >= 0 ? static_cast<const TI*>(a.q) + row * a.q_stride + head * kv.hd : nullptr, kv.hd, rule.mul);
 
-  constexpr float LIFT = __is_same(TC, _Float16) ? 15.0f : 0.0f;
+  // over halves the shares are taken against 2^-8 of a maximum that may be
+  // exceeded 2^7 times before it is raised: what is down to 2^-22 of it then stays
+  // a normal half
+  constexpr float LIFT = __is_same(TC, _Float16) ? 8.0f : 0.0f, SLACK = 7.0f;
   float m = MAX_START, z = 0.0f;
   // Rows of one block differ in position by up to 15 tokens: a step that lies
   // before all of them and inside every window needs no masks.
@@ -258,8 +261,9 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
     for (int T = 0; T < 2; ++T) {
       const f32x4 x = tile.scores(T);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[4 * T + i] = score_of(rule, x[i], tile.mul);
+      for (int i = 0; i < 4; ++i) s[4 * T + i] = x[i];
     }
+    scores_of<8>(rule, s, tile.mul);
     if (a.rl.slopes) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) s[i] -= slope * fabsf(static_cast<float>(pos - (p0 + 16 * (i >> 2) + 4 * g + (i & 3))));
@@ -278,10 +282,8 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
       *reinterpret_cast<f32x4*>(sc_row + p0 + 4 * g) = f32x4{s[0], s[1], s[2], s[3]};
       *reinterpret_cast<f32x4*>(sc_row + p0 + 16 + 4 * g) = f32x4{s[4], s[5], s[6], s[7]};
     }
-    // over halves the shares are taken against 2^-15 of the largest: what is
-    // down to 2^-29 of it then stays a normal half
     float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7]))) - LIFT;
-    if (__any(top > m)) {
+    if (__any(top > m + SLACK)) {
       top = fmaxf(top, lane_xor16(top));
       top = fmaxf(top, lane_xor32(top));
       const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
@@ -491,9 +493,9 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
   p.n_blocks = static_cast<int>((rows + p.block_rows - 1) / p.block_rows);
   const int64_t table = static_cast<int64_t>(bt.max_pages) << kv.page_shift;
   int64_t span = std::min<int64_t>(bt.max_len, table);
-  p.score_len = static_cast<int>((span + 31) / 32 * 32);
-  // rows of a block are at most block_rows positions apart, lo goes down to a multiple of 32
-  if (rl.window > 0 && !rl.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(rl.window) + p.block_rows + 32);
+  p.score_len = static_cast<int>((span + 63) / 64 * 64);
+  // rows of a block are at most block_rows positions apart, lo goes down to a multiple of 64
+  if (rl.window > 0 && !rl.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(rl.window) + p.block_rows + 64);
   span = std::max<int64_t>(span, 1);
   const int64_t blocks = static_cast<int64_t>(bt.n_seq) * kv.n_kv_heads * p.n_blocks;
   if (p.few) {

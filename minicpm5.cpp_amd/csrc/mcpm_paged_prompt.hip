@@ -93,6 +93,34 @@ struct Prompt16 {
       }
     }
   }
+  // The same for a whole tile whose pages hold 16 positions or more: the rows of a
+  // wave's load are in one page, so that its address is a scalar base(position) and
+  // an offset that a lane keeps.
+  uint32_t k_lane, v_lane;
+  __device__ __forceinline__ void set_lanes(int hd, uint32_t pos_stride) {
+    const int lane = threadIdx.x & 63;
+    k_lane = (lane / (DP / 8) * pos_stride + min(lane % (DP / 8) * 8, hd - 8)) * 2;
+    v_lane = (4 * (lane >> 4) * pos_stride) * 2;
+  }
+  template <class Base>
+  __device__ __forceinline__ void load_whole(const TC* kc, const TC* vc, int p0, int wave, int hd, int64_t pos_stride, const Base& base) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const char* p = reinterpret_cast<const char*>(kc + base(p0 + (wave * 64 + 256 * i) / (DP / 8)));
+      gk[i] = *reinterpret_cast<const u32x4*>(p + k_lane);
+    }
+    const TC* v = vc + base(p0 + 16 * wave);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const char* row = reinterpret_cast<const char*>(v + r * pos_stride);
+#pragma unroll
+      for (int it = 0; it < NI; ++it) {
+        const char* p = row + (v_lane + 2 * min(E * (16 * it + static_cast<int>(threadIdx.x & 15)), hd - E));
+        if constexpr (E == 8) *reinterpret_cast<u32x4*>(gv[it][r]) = *reinterpret_cast<const u32x4*>(p);
+        else *reinterpret_cast<u32x2*>(gv[it][r]) = *reinterpret_cast<const u32x2*>(p);
+      }
+    }
+  }
   __device__ __forceinline__ void store(char* buf) const {
     const int tid = threadIdx.x;
 #pragma unroll
@@ -193,6 +221,20 @@ struct PromptTile<float, float, DP> {
       gv[i] = *reinterpret_cast<const u32x4*>(vc + at);
     }
   }
+  uint32_t lane_off;
+  __device__ __forceinline__ void set_lanes(int hd, uint32_t pos_stride) {
+    const int lane = threadIdx.x & 63;
+    lane_off = (lane / (DP / 4) * pos_stride + min(lane % (DP / 4) * 4, hd - 4)) * 4;
+  }
+  template <class Base>
+  __device__ __forceinline__ void load_whole(const float* kc, const float* vc, int p0, int wave, int, int64_t, const Base& base) {
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int64_t at = base(p0 + (wave * 64 + 256 * i) / (DP / 4));
+      gk[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(kc + at) + lane_off);
+      gv[i] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const char*>(vc + at) + lane_off);
+    }
+  }
   __device__ __forceinline__ void store(char* buf) const {
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
@@ -251,10 +293,10 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
   __shared__ __attribute__((aligned(16))) int s_doc[2][KT];
   __shared__ unsigned char s_bad[PR_ROWS];
   __shared__ unsigned s_tiles;
-  __shared__ int s_docs[2];
+  __shared__ int s_docs[2], s_plain[2];
   extern __shared__ int64_t s_off[];
   const PagedView& kv = a.kv;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, n32 = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), n32 = lane & 31, half = lane >> 5;
   // work groups of one sequence and kv head are `pairs` apart, which keeps them on
   // one XCD where pairs divides 8 or the reverse; the rows with the most keys come first
   const int pairs = a.bt.n_seq * kv.n_kv_heads;
@@ -295,6 +337,11 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
     atomicMax(&s_docs[1], rr.doc);
   }
 
+  // a wave's rows in a page, and their offsets in 32 bits
+  const bool whole_pages = kv.page_mask >= 15 && kv.pos_stride <= 1 << 24;
+  tile.set_lanes(kv.hd, static_cast<uint32_t>(kv.pos_stride));
+  const bool all_rows = !__any(row_in && rr.pos < 0);  // none of no document or before the start
+
   float m = MAX_START, z = 0.0f;
   for (int seg = c0; seg < c1; seg += SEG) {
     const int seg_end = min(c1, seg + SEG);
@@ -320,42 +367,69 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
       return s_off[(j >> kv.page_shift) - first_page] +
              static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(j & kv.page_mask)) * static_cast<uint32_t>(kv.pos_stride));
     };
+    // the same of a position that the wave shares, not past the end
+    auto base = [&](int j) -> int64_t {
+      const uint64_t e = static_cast<uint64_t>(s_off[(j >> kv.page_shift) - first_page]);
+      const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(e)), hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(e >> 32));
+      return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo) + (j & kv.page_mask) * kv.pos_stride;
+    };
+    auto load = [&](int p0) {
+      if (whole_pages && p0 + KT <= seg_end) tile.load_whole(kc, vc, p0, wv, kv.hd, kv.pos_stride, base);
+      else tile.load(kc, vc, p0, kv.hd, offset);
+    };
     int cur = __builtin_ctz(todo), buf = 0;
     todo &= todo - 1;
-    tile.load(kc, vc, seg + cur * KT, kv.hd, offset);
+    load(seg + cur * KT);
     tile.store(s_tile[0]);
-    if (docs && tid < KT) s_doc[0][tid] = docs[min(seg + cur * KT + tid, seg_end - 1)];
+    auto stage_docs = [&](int at, int p0) {
+      if (!docs || wv) return;
+      const int d = lane < KT ? docs[min(p0 + lane, seg_end - 1)] : s_docs[0];
+      if (lane < KT) s_doc[at][lane] = d;
+      const bool plain = !__any(d != s_docs[0]);
+      if (lane == 0) s_plain[at] = plain;
+    };
+    stage_docs(0, seg + cur * KT);
     for (;;) {
       const int next = todo ? __builtin_ctz(todo) : -1;
       todo &= todo - 1;
       __syncthreads();
-      if (next >= 0) tile.load(kc, vc, seg + next * KT, kv.hd, offset);
+      if (next >= 0) load(seg + next * KT);
       const int p0 = seg + cur * KT;
+      // one document in the tile and in the rows: nothing to tell apart
+      const bool doc_masks = docs && !(s_docs[0] == s_docs[1] && s_plain[buf]);
       if (wave_in && (p0 <= last || p0 < prefix) && !(a.rl.window > 0 && first - (p0 + KT - 1) >= a.rl.window)) {
 #pragma unroll
         for (int sub = 0; sub < KT / 32; ++sub) {
           const int pp = p0 + 32 * sub;  // the lane: positions pp + 8 (i / 4) + 4 half + i % 4
           f32x16 s = tile.scores(s_tile[buf], sub);
+          const bool masked = doc_masks || !all_rows || bad_pages || pp + 31 > first || pp + 32 > seg_end || (a.rl.window > 0 && last - pp >= a.rl.window);
+          const bool shaped = rule.capped || a.rl.slopes || masked || !(rule.mul > 0.0f);  // the same for the wave
+          float scale = tile.mul;
+          if (shaped) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) s[i] = score_of(rule, s[i], tile.mul);
-          if (a.rl.slopes) {
+            for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(s[i]));  // nothing of this ahead of the branch
+            scale = 1.0f;
+            scores_of<16>(rule, s, tile.mul);
+            if (a.rl.slopes) {
+              const float far = static_cast<float>(pos - (pp + 4 * half));
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] -= slope * fabsf(static_cast<float>(pos - (pp + 8 * (i / 4) + 4 * half + i % 4)));
-          }
-          if (docs || bad_pages || pp + 31 > first || pp + 32 > seg_end || (a.rl.window > 0 && last - pp >= a.rl.window)) {
+              for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope, fabsf(far - static_cast<float>(8 * (i / 4) + i % 4)), s[i]);
+            }
+            if (masked) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int o = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, j = p0 + o;
-              bool ok = (j < seg_end) & ((j <= rr.pos) | (j < rr.prefix)) & (rr.pos - j < rr.window);
-              if (docs) ok &= s_doc[buf][o] == rr.doc;
-              if (bad_pages) ok &= page_of(a.bt, kv, b, min(j, seg_end - 1)) >= 0;
-              s[i] = ok ? s[i] : -__builtin_inff();
+              for (int i = 0; i < 16; ++i) {
+                const int o = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, j = p0 + o;
+                bool ok = (j < seg_end) & ((j <= rr.pos) | (j < rr.prefix)) & (rr.pos - j < rr.window);
+                if (docs) ok &= s_doc[buf][o] == rr.doc;
+                if (bad_pages) ok &= page_of(a.bt, kv, b, min(j, seg_end - 1)) >= 0;
+                s[i] = ok ? s[i] : -__builtin_inff();
+              }
             }
           }
           float top = s[0];
 #pragma unroll
           for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-          top -= LIFT;
+          top = __builtin_fmaf(top, scale, -LIFT);
           if (__any(top > m + SLACK)) {
             top = fmaxf(top, lane_xor32(top));
             const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
@@ -367,7 +441,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
           float p[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(s[i] - m);
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -m));
             z += p[i];
           }
           tile.add(s_tile[buf], sub, p);
@@ -375,7 +449,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
       }
       if (next < 0) break;
       tile.store(s_tile[buf ^ 1]);
-      if (docs && tid < KT) s_doc[buf ^ 1][tid] = docs[min(seg + next * KT + tid, seg_end - 1)];
+      stage_docs(buf ^ 1, seg + next * KT);
       cur = next;
       buf ^= 1;
     }

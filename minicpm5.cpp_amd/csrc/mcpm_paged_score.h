@@ -56,19 +56,23 @@ __device__ __forceinline__ void split_terms(const float (&x)[M], typename Half<T
   }
 }
 
-// tanh: by its series to x^11 below 0.3 (the next term is 2e-9 of it), from
-// exp(2x) above.
-__device__ __forceinline__ float tanh_f32(float x) {
-  const float a = fabsf(x), x2 = x * x;
+// tanh below 0.3 by its series to x^11 (the next term is 2e-9 of it).
+constexpr float TANH_SERIES = 0.3f;
+__device__ __forceinline__ float tanh_small(float x) {
+  const float x2 = x * x;
   float p = -8.8632355299e-3f;
   p = __builtin_fmaf(p, x2, 2.1869488536e-2f);
   p = __builtin_fmaf(p, x2, -5.3968253968e-2f);
   p = __builtin_fmaf(p, x2, 1.3333333333e-1f);
   p = __builtin_fmaf(p, x2, -3.3333333333e-1f);
-  const float small = __builtin_fmaf(x * x2, p, x);
+  return __builtin_fmaf(x * x2, p, x);
+}
+// Above from exp(2x).
+__device__ __forceinline__ float tanh_f32(float x) {
+  const float a = fabsf(x);
   const float e = __builtin_amdgcn_exp2f(a * (2.0f * LOG2E));
   const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
-  return a < 0.3f ? small : __builtin_copysignf(large, x);
+  return a < TANH_SERIES ? tanh_small(x) : __builtin_copysignf(large, x);
 }
 
 // Scores in units of log2: p = 2^(s - m).  `mul` takes a raw product q.k to the
@@ -84,6 +88,25 @@ __device__ __forceinline__ ScoreRule score_rule(const RuleView& rl) {
 __device__ __forceinline__ float score_of(const ScoreRule& sr, float dot, float mul) {
   const float s = dot * mul;
   return sr.capped ? sr.cap * tanh_f32(s) : s;
+}
+
+// N scores of a lane at once: caps are seldom near, so a wave whose arguments are
+// all small takes the series alone.
+template <int N, class Dots>
+__device__ __forceinline__ void scores_of(const ScoreRule& sr, Dots& s, float mul) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) s[i] *= mul;
+  if (!sr.capped) return;
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(s[i]));
+  if (__any(!(top < TANH_SERIES))) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = sr.cap * tanh_f32(s[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = sr.cap * tanh_small(s[i]);
+  }
 }
 
 // A row's place under the rules; pos < 0 (no row, or one of no document) sees nothing.
@@ -107,7 +130,7 @@ __device__ __forceinline__ bool seen(const RuleView& rl, const RowRule& r, int b
   return ok;
 }
 
-// Positions [lo, hi) that rows at pos0 .. pos1 may see, lo at a multiple of 32.
+// Positions [lo, hi) that rows at pos0 .. pos1 may see, lo at a multiple of 64.
 struct KeyRange {
   int lo, hi;
 };
@@ -117,7 +140,7 @@ __device__ __forceinline__ KeyRange key_range(const RuleView& rl, int b, int pos
   if (rl.prefix) hi = max(hi, rl.prefix[b]);
   hi = min(hi, len);
   if (pos1 < 0) hi = 0;
-  return KeyRange{lo & ~31, hi};
+  return KeyRange{lo & ~63, hi};
 }
 
 // A call as its kernels see it.  A row block is `block_rows` rows of a sequence

@@ -217,6 +217,20 @@ def test_prompt_long_past(ctx, t, io):
     check_attention(ctx, "long past", (4, 1, 128), t, io, [2200, 90], [30, 90], page=64, seed=3, order="hpd", pad=1)
 
 
+@pytest.mark.parametrize("t,io", TYPES, ids=IDS)
+def test_prompt_documents_of_many_tiles(ctx, t, io):
+    """Documents longer than a tile of keys, so that tiles hold one alone; rows of no document between rows of one,
+    in the same block of rows."""
+    n = 400
+    d = np.zeros((2, n), np.int32)
+    d[0, 150:] = 1
+    d[0, 333:] = 7
+    d[0, [140, 141, 329, 395, 396, 397, 398, 399]] = -1
+    d[1, -20:] = -1
+    check_attention(ctx, "long documents", (8, 2, 64), t, io, [n, n - 30], [n, 260], page=64, rules=dict(docs=d), seed=15)
+    check_attention(ctx, "long documents", (16, 1, 128), t, io, [n, 200], [90, 33], page=64, rules=dict(docs=d, softcap=20.0), weight=True, seed=16)
+
+
 # ---------------------------------------------------------- what no row sees
 
 def spoil(bad):
