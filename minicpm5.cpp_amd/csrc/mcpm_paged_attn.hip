@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   const int64_t row = sr.r0 + t;
   const int pos = fb.pos0 + t;
   const ScoreRule rule = score_rule(a.rl);
-  const RowRule rr = row_rule(a.rl, b, row_in ? pos : -1);
+  const RowRule rr = row_rule(a.rl, b, row_in ? pos : -1, c1);
   const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
   const TC* kc = reinterpret_cast<const TC*>(kv.k) + kh * kv.head_stride;
   const TC* vc = reinterpret_cast<const TC*>(kv.v) + kh * kv.head_stride;
@@ -269,13 +269,16 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
       for (int i = 0; i < 8; ++i) s[i] -= slope * fabsf(static_cast<float>(pos - (p0 + 16 * (i >> 2) + 4 * g + (i & 3))));
     }
     if (!plain || p0 + FEW_STEP - 1 > fb.first || p0 + FEW_STEP > c1 || (a.rl.window > 0 && fb.last - p0 >= a.rl.window)) {
+      const int j0 = p0 + 4 * g - rr.lo;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int j = p0 + 16 * (i >> 2) + 4 * g + (i & 3);
-        const int jc = min(j, c1 - 1);
-        bool ok = (j < c1) & seen(a.rl, rr, b, jc);
-        if (bad_pages) ok &= page_of(a.bt, kv, b, jc) >= 0;
-        s[i] = ok ? s[i] : -__builtin_inff();
+      for (int i = 0; i < 8; ++i) s[i] = static_cast<unsigned>(j0 + 16 * (i >> 2) + (i & 3)) < rr.span ? s[i] : -__builtin_inff();
+      if (a.rl.docs || bad_pages) {  // the 32 positions' tags, one a lane
+        const int tag = tag_of(a.rl, a.bt, kv, b, min(p0 + (lane & 31), c1 - 1), bad_pages);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int x = __shfl(tag, 16 * (i >> 2) + 4 * g + (i & 3));
+          s[i] = x == rr.tag ? s[i] : -__builtin_inff();
+        }
       }
     }
     if (sc_row) {
@@ -355,64 +358,60 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   __syncthreads();
   if (!s_bad) return;
   // Something infinite or NaN came up: perhaps only a share of 0 times it.
-  for (int i = 0; i < FEW_ROWS && rb * FEW_ROWS + i < fb.r_end; ++i) {
-    const int ri = rb * FEW_ROWS + i, ti = ri / a.group, hi = kh * a.group + ri - ti * a.group;
-    float2 mz;
-    const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + ti, hi, fb.pos0 + ti, c0, c1, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0], &mz);
-    const int64_t ai = part_index(a, b, ti, hi, split);
-    if (tid < kv.hd) {
-      if (final) static_cast<TI*>(a.out)[(sr.r0 + ti) * a.out_stride + hi * kv.hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
-      else a.part_o[ai * kv.hd + tid] = o;
-    }
-    if (tid == 0 && a.part_mz) a.part_mz[ai] = mz;
-  }
+  exact_rows<TC, TI>(b, kh, rb, split, FEW_ROWS, nullptr, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0]);
 }
 
-// The splits' maxima and sums of a row joined, by a wave.
-__device__ __forceinline__ float2 join_mz(const float2* mz, int n) {
-  const int lane = threadIdx.x & 63;
-  float M = MAX_START;
-  for (int i = lane; i < n; i += 64) M = fmaxf(M, mz[i].x);
-  M = wave_max(M);
-  float Z = 0.0f;
-  for (int i = lane; i < n; i += 64) Z += mz[i].y * __builtin_amdgcn_exp2f(mz[i].x - M);
-  for (int s = 32; s; s >>= 1) Z += __shfl_xor(Z, s);
-  return make_float2(M, Z);
-}
 __device__ __forceinline__ int active_splits(const PagedCall& a, const KeyRange& k) {
   return k.hi > k.lo ? (k.hi - k.lo + a.chunk - 1) / a.chunk : 1;
 }
 
-// A work group per (new token, head): the splits' partials into the output,
-// 256 / (DP/4) of them at a time.
-template <typename TI, int DP>
+// The splits' partials of ROWS (new token, head)s into the output, a work group:
+// DP/4 lanes hold a row's elements, 256 / (DP/4) / ROWS of them take its splits in turn.
+template <typename TI, int DP, int ROWS>
 __global__ void __launch_bounds__(256) k_attention_join(const PagedCall a) {
-  constexpr int LP = DP / 4, GR = 256 / LP;
-  __shared__ f32x4 s_acc[GR][LP];
+  constexpr int LP = DP / 4, GR = 256 / LP / ROWS;
+  __shared__ f32x4 s_acc[ROWS][GR][LP];
+  __shared__ float2 s_mz[ROWS][GR];
   const int b = blockIdx.y, tid = threadIdx.x, hd = a.kv.hd;
+  const int e = tid % LP, g = tid / LP % GR, i = tid / LP / GR;
   const SeqRows sr = seq_rows(a.bt, b);
-  const int t = blockIdx.x / a.n_heads, head = blockIdx.x % a.n_heads;
-  if (t >= sr.n) return;
-  const int rb = (t * a.group + head % a.group) / a.block_rows;
-  const int n = active_splits(a, row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b)).keys);
-  const int64_t at = part_index(a, b, t, head, 0);
-  const float2 mz = join_mz(a.part_mz + at, n);
-  const int d = tid % LP * 4;
+  const int item = blockIdx.x * ROWS + i, t = item / a.n_heads, head = item - t * a.n_heads;
+  const bool in = t < sr.n;
   f32x4 acc{0, 0, 0, 0};
-  if (d < hd)
-    for (int i = tid / LP; i < n; i += GR) {
-      const float2 x = a.part_mz[at + i];
-      if (x.y != 0.0f) acc += __builtin_amdgcn_exp2f(x.x - mz.x) * *reinterpret_cast<const f32x4*>(a.part_o + (at + i) * hd + d);
+  float2 mz = make_float2(MAX_START, 0.0f);
+  int64_t at = 0;
+  if (in) {
+    const int rb = (t * a.group + head % a.group) / a.block_rows;
+    const int n = active_splits(a, row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b)).keys);
+    at = part_index(a, b, t, head, 0);
+    for (int k = g; k < n; k += GR) {
+      const float2 x = a.part_mz[at + k];
+      if (x.y == 0.0f) continue;
+      const f32x4 o = e * 4 < hd ? *reinterpret_cast<const f32x4*>(a.part_o + (at + k) * hd + e * 4) : f32x4{0, 0, 0, 0};
+      const float m = fmaxf(mz.x, x.x), f = __builtin_amdgcn_exp2f(mz.x - m), w = __builtin_amdgcn_exp2f(x.x - m);
+      acc = f * acc + w * o;
+      mz = make_float2(m, f * mz.y + w * x.y);
     }
-  s_acc[tid / LP][tid % LP] = acc;
-  __syncthreads();
-  if (tid == 0 && a.kv.weight) a.part_mz[at] = mz;
-  if (tid >= LP || d >= hd) return;
-  for (int i = 1; i < GR; ++i) acc += s_acc[i][tid];
+  }
+  if constexpr (GR > 1) {
+    s_acc[i][g][e] = acc;
+    if (e == 0) s_mz[i][g] = mz;
+    __syncthreads();
+    if (g) return;
+    for (int k = 1; k < GR; ++k) {
+      const float2 x = s_mz[i][k];
+      const float m = fmaxf(mz.x, x.x), f = __builtin_amdgcn_exp2f(mz.x - m), w = __builtin_amdgcn_exp2f(x.x - m);
+      acc = f * acc + w * s_acc[i][k][e];
+      mz = make_float2(m, f * mz.y + w * x.y);
+    }
+  }
+  if (!in) return;
+  if (e == 0 && a.kv.weight) a.part_mz[at] = mz;
+  if (e * 4 >= hd) return;
   const float inv = mz.y == 0.0f ? 0.0f : 1.0f / mz.y;
-  TI* dst = static_cast<TI*>(a.out) + (sr.r0 + t) * a.out_stride + head * hd + d;
+  TI* dst = static_cast<TI*>(a.out) + (sr.r0 + t) * a.out_stride + head * hd + e * 4;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) dst[i] = static_cast<TI>(acc[i] * inv);
+  for (int k = 0; k < 4; ++k) dst[k] = static_cast<TI>(acc[k] * inv);
 }
 
 // The positions' weights from the scores: a lane per position sums its rows in order.
@@ -462,8 +461,8 @@ __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
   float sum = 0.0f;
   for (int t = 0; t < sr.n; ++t) {
     const int pos = len - sr.given + t;
-    const RowRule rr = row_rule(a.rl, b, pos);
-    if (!seen(a.rl, rr, b, j)) continue;
+    const RowRule rr = row_rule(a.rl, b, pos, len);
+    if (!in_span(rr, j) || tag_of(a.rl, a.bt, kv, b, j, false) != rr.tag) continue;
     for (int h = kh * a.group; h < kh * a.group + a.group; ++h) {
       const TI* q = static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + h * hd;
       float d = 0.0f;
@@ -530,13 +529,20 @@ hipError_t launch_attention_few(const PagedCall& a, int kv_type, int io_type, hi
   return f32 ? few<__bf16, float>(a, s) : few<__bf16, __bf16>(a, s);
 }
 
-template <typename TI>
-hipError_t join(const PagedCall& a, hipStream_t s) {
-  const dim3 grid(a.bt.max_new * a.n_heads, a.bt.n_seq);
-  if (a.kv.hd <= 64) hipLaunchKernelGGL((k_attention_join<TI, 64>), grid, dim3(256), 0, s, a);
-  else if (a.kv.hd <= 128) hipLaunchKernelGGL((k_attention_join<TI, 128>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_attention_join<TI, 256>), grid, dim3(256), 0, s, a);
+template <typename TI, int DP>
+hipError_t join(const PagedCall& a, int n_cu, hipStream_t s) {
+  constexpr int LP = DP / 4, MOST = 256 / LP;
+  const int items = a.bt.max_new * a.n_heads;
+  // rows side by side where that leaves a work group per CU, else the splits
+  if (static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu)
+    hipLaunchKernelGGL((k_attention_join<TI, DP, MOST>), dim3((items + MOST - 1) / MOST, a.bt.n_seq), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((k_attention_join<TI, DP, 1>), dim3(items, a.bt.n_seq), dim3(256), 0, s, a);
   return hipGetLastError();
+}
+template <typename TI>
+hipError_t join(const PagedCall& a, int n_cu, hipStream_t s) {
+  return a.kv.hd <= 64 ? join<TI, 64>(a, n_cu, s) : a.kv.hd <= 128 ? join<TI, 128>(a, n_cu, s) : join<TI, 256>(a, n_cu, s);
 }
 
 template <typename TC, typename TI>
@@ -563,7 +569,7 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
   hipError_t e = p.few ? launch_attention_few(a, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
   if (e != hipSuccess) return e;
   if (p.n_splits > 1) {
-    e = io_type == MCPM_TYPE_F32 ? join<float>(a, s) : io_type == MCPM_TYPE_F16 ? join<_Float16>(a, s) : join<__bf16>(a, s);
+    e = io_type == MCPM_TYPE_F32 ? join<float>(a, n_cu, s) : io_type == MCPM_TYPE_F16 ? join<_Float16>(a, n_cu, s) : join<__bf16>(a, n_cu, s);
     if (e != hipSuccess) return e;
   }
   if (!kv.weight || !p.score_len) return hipSuccess;

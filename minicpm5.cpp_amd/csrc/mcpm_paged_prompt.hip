@@ -19,6 +19,15 @@ namespace {
 
 constexpr int PR_ROWS = 128;
 
+// All of `x` in registers here: without it the compiler gives every matrix
+// instruction an LDS read of its own to wait for.
+template <int N, typename T>
+__device__ __forceinline__ void all_here(T (&x)[N]) {
+  static_assert(N % 4 == 0);
+#pragma unroll
+  for (int i = 0; i < N; i += 4) asm volatile("" : "+v"(x[i]), "+v"(x[i + 1]), "+v"(x[i + 2]), "+v"(x[i + 3]));
+}
+
 // 16-bit caches: tiles of 64 positions.
 template <typename TC, typename TI, int DP>
 struct Prompt16 {
@@ -39,16 +48,24 @@ struct Prompt16 {
   // Rows of 32 bits over halves are brought to a top exponent of 8 by a power of
   // two, so that neither term leaves a half's range; products take it back.
   __device__ __forceinline__ void load_q(const TI* row, int hd, float score_mul) {
+    typedef TI Row __attribute__((ext_vector_type(8)));
     const int h = (threadIdx.x >> 5) & 1;
-    int e = 0;
+    Row x[KS];
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      const bool in = row && 16 * s + 8 * h < hd;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[s][i] = static_cast<TI>(0.0f);
+      if (in) x[s] = *reinterpret_cast<const Row*>(row + 16 * s + 8 * h);
+    }
     mul = score_mul;
+    int e = 0;
     if (NT == 2) {
-      float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (row && 16 * s + 8 * h < hd) top = fmaxf(top, fabsf(static_cast<float>(row[16 * s + 8 * h + i])));
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(static_cast<float>(x[s][i])));
       top = fmaxf(top, lane_xor32(top));
       if (top > 0.0f && top < __builtin_inff()) {
         e = 9 - __builtin_amdgcn_frexp_expf(top);
@@ -57,15 +74,11 @@ struct Prompt16 {
     }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      float x[8];
+      float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = row && 16 * s + 8 * h < hd ? static_cast<float>(row[16 * s + 8 * h + i]) : 0.0f;
-      if (NT == 2) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = ldexpf(x[i], e);
-      }
+      for (int i = 0; i < 8; ++i) y[i] = NT == 2 ? ldexpf(static_cast<float>(x[s][i]), e) : static_cast<float>(x[s][i]);
       V8 t[NT];
-      split_terms<TC, NT>(x, t);
+      split_terms<TC, NT>(y, t);
 #pragma unroll
       for (int n = 0; n < NT; ++n) q[n][s] = t[n];
     }
@@ -140,23 +153,70 @@ struct Prompt16 {
             u32x2{__builtin_amdgcn_perm(r[1][j / 2], r[0][j / 2], sel), __builtin_amdgcn_perm(r[3][j / 2], r[2][j / 2], sel)};
       }
   }
-  __device__ __forceinline__ f32x16 scores(const char* buf, int sub) const {
+  // Operands of the products, four 16-byte reads ahead of their use in a ring: of K's
+  // KS steps of 16 elements, of V's KS tiles of 32 elements and 16 positions.
+  static constexpr int RING = 4;
+  V8 k[RING], v[RING];
+  static_assert(KS == 2 * NO && KS >= RING);
+  __device__ __forceinline__ const char* k_at(const char* buf, int sub) const {
     const int m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
-    const char* k = buf + (32 * sub + m) * K_STRIDE + h * 16;
-    f32x16 s;
+    return buf + (32 * sub + m) * K_STRIDE + h * 16;
+  }
+  __device__ __forceinline__ const char* v_at(const char* buf, int sub) const {
+    const int m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+    return buf + KT * K_STRIDE + m * V_STRIDE + sub * 64 + h * 16;
+  }
+  __device__ __forceinline__ void read_k(const char* at, int i) { k[i % RING] = *reinterpret_cast<const V8*>(at + i * 32); }
+  __device__ __forceinline__ void read_v(const char* at, int i) { v[i % RING] = *reinterpret_cast<const V8*>(at + i % NO * 32 * V_STRIDE + i / NO * 32); }
+  __device__ __forceinline__ void begin_k(const char* at) {
+#pragma unroll
+    for (int i = 0; i < RING; ++i) read_k(at, i);
+  }
+  __device__ __forceinline__ void score_step(f32x16& s, const char* at, int i) {
+#pragma unroll
+    for (int n = NT - 1; n >= 0; --n) s = Half<TC>::mma32(k[i % RING], q[n][i], s);
+    if (i + RING < KS) read_k(at, i + RING);
+  }
+  // Scores of the positions whose K begin_k began to read.
+  __device__ __forceinline__ void scores(f32x16& s, const char* at) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      const V8 a = *reinterpret_cast<const V8*>(k + i * 32);
-#pragma unroll
-      for (int n = NT - 1; n >= 0; --n) s = Half<TC>::mma32(a, q[n][i], s);
+      score_step(s, at, i);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    return s;
   }
-  __device__ __forceinline__ void add(const char* buf, int sub, const float (&p)[16]) {
-    const int m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
-    const char* v = buf + KT * K_STRIDE + m * V_STRIDE + sub * 64 + h * 16;
+  // A tile's 64 positions in the order in which its two halves overlap best.  Program
+  // order is kept (a matrix instruction occupies its unit for 32 cycles, in which the
+  // wave issues the vector instructions that follow it): the scores of the second half
+  // between the shares of the first, then the first half's outputs between the shares of
+  // the second.
+  static constexpr int PER = 16 / KS;  // shares to a matrix step
+  __device__ __forceinline__ void share(const f32x16& s, float (&p)[16], float scale, float m, float& z, int i) const {
+#pragma unroll
+    for (int e = i * PER; e < (i + 1) * PER; ++e) {
+      p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e], scale, -m));
+      z += p[e];
+    }
+  }
+  __device__ __forceinline__ void scores_and_shares(f32x16& n, const char* k_base, const f32x16& s, float (&p)[16], float scale, float m, float& z,
+                                                    const char* v_base) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) n[i] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < KS; ++i) {
+      score_step(n, k_base, i);
+      if (i >= KS - RING) read_v(v_base, i - (KS - RING));
+      share(s, p, scale, m, z, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  // Outputs of the shares p (V from v_base, its first reads begun); with MORE the
+  // shares of s meanwhile, into p2, and the first reads of V at v_after.
+  template <bool MORE>
+  __device__ __forceinline__ void outputs(const float (&p)[16], const char* v_base, const f32x16& s, float (&p2)[16], float scale, float m, float& z,
+                                          const char* v_after) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       float x[8];
@@ -166,9 +226,15 @@ struct Prompt16 {
       split_terms<TC, NT>(x, t);
 #pragma unroll
       for (int j = 0; j < NO; ++j) {
-        const V8 a = *reinterpret_cast<const V8*>(v + j * 32 * V_STRIDE + ks * 32);
+        const int i = ks * NO + j;
 #pragma unroll
-        for (int n = NT - 1; n >= 0; --n) o[j] = Half<TC>::mma32(a, t[n], o[j]);
+        for (int c = NT - 1; c >= 0; --c) o[j] = Half<TC>::mma32(v[i % RING], t[c], o[j]);
+        if (i + RING < KS) read_v(v_base, i + RING);
+        if constexpr (MORE) {
+          if (i >= KS - RING) read_v(v_after, i - (KS - RING));
+          share(s, p2, scale, m, z, i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
@@ -244,34 +310,47 @@ struct PromptTile<float, float, DP> {
       *reinterpret_cast<u32x4*>(p + KT * STRIDE) = gv[i];
     }
   }
-  __device__ __forceinline__ f32x16 scores(const char* buf, int) const {
+  __device__ __forceinline__ void scores(f32x16& s, const char* buf) const {
     const int m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
     const char* k = buf + m * STRIDE + h * 16;
-    f32x16 s;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s[i] = 0.0f;
 #pragma unroll
-    for (int i = 0; i < KS; ++i) {
-      const f32x4 a = *reinterpret_cast<const f32x4*>(k + i * 32);
+    for (int i0 = 0; i0 < KS; i0 += 8) {
+      f32x4 a[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[c], q[i][c], s, 0, 0, 0);
+      for (int i = 0; i < 8; ++i) a[i] = *reinterpret_cast<const f32x4*>(k + (i0 + i) * 32);
+      all_here(a);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][c], q[i0 + i][c], s, 0, 0, 0);
     }
-    return s;
   }
-  __device__ __forceinline__ void add(const char* buf, int, const float (&p)[16]) {
-    const int m = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
-    const char* v = buf + KT * STRIDE + 4 * h * STRIDE + m * W * 4;
+  __device__ __forceinline__ void step(const f32x16& s, float scale, float m, float& z, const char* buf) {
+    typedef float VecW __attribute__((ext_vector_type(W)));
+    const int m32 = threadIdx.x & 31, h = (threadIdx.x >> 5) & 1;
+    const char* v = buf + KT * STRIDE + 4 * h * STRIDE + m32 * W * 4;
+    float p[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const char* row = v + (8 * (i / 4) + i % 4) * STRIDE;
+      p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -m));
+      z += p[i];
+    }
 #pragma unroll
-      for (int t = 0; t < NO / W; ++t) {
-        float x[W];
-        if constexpr (W == 4) *reinterpret_cast<f32x4*>(x) = *reinterpret_cast<const f32x4*>(row + t * 32 * W * 4);
-        else *reinterpret_cast<u32x2*>(x) = *reinterpret_cast<const u32x2*>(row + t * 32 * W * 4);
+    for (int i0 = 0; i0 < 16; i0 += 4) {
+      VecW x[4 * NO / W];
 #pragma unroll
-        for (int c = 0; c < W; ++c) o[t * W + c] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[c], p[i], o[t * W + c], 0, 0, 0);
-      }
+      for (int i = 0; i < 4 * NO / W; ++i)
+        x[i] = *reinterpret_cast<const VecW*>(v + (2 * i0 + i / (NO / W)) * STRIDE + i % (NO / W) * 32 * W * 4);
+      all_here(x);
+#pragma unroll
+      for (int i = 0; i < 4 * NO / W; ++i)
+#pragma unroll
+        for (int c = 0; c < W; ++c) {
+          const int j = i % (NO / W) * W + c;
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(x[i][c], p[i0 + i / (NO / W)], o[j], 0, 0, 0);
+        }
     }
   }
   static constexpr int RUN = W, RUNS = DP / (2 * W);
@@ -282,18 +361,24 @@ struct PromptTile<float, float, DP> {
   __device__ __forceinline__ float run(int c, int x) const { return o[c / 16 * W + x][c % 16]; }
 };
 
+// Waves per SIMD: two where the registers suffice.
 template <typename TC, typename TI, int DP>
-__global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(const PagedCall a) {
+constexpr int prompt_waves() {
+  return DP <= 64 || (DP <= 128 && Terms<TC, TI>::N == 1) ? 2 : 1;
+}
+
+template <typename TC, typename TI, int DP>
+__global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention_prompt(const PagedCall a) {
   typedef PromptTile<TC, TI, DP> Tile;
   constexpr int KT = Tile::KT, SEG = 32 * KT;
   // over halves the shares are taken against 2^-8 of a maximum that may be
   // exceeded 2^7 times before it is raised
   constexpr float LIFT = __is_same(TC, _Float16) ? 8.0f : 0.0f, SLACK = 7.0f;
   __shared__ __attribute__((aligned(16))) char s_tile[2][Tile::BYTES];
-  __shared__ __attribute__((aligned(16))) int s_doc[2][KT];
+  __shared__ __attribute__((aligned(16))) int s_tag[2][KT];
   __shared__ unsigned char s_bad[PR_ROWS];
   __shared__ unsigned s_tiles;
-  __shared__ int s_docs[2], s_plain[2];
+  __shared__ int s_tags[2], s_plain[2];
   extern __shared__ int64_t s_off[];
   const PagedView& kv = a.kv;
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), n32 = lane & 31, half = lane >> 5;
@@ -317,7 +402,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
   const int pos = fb.pos0 + t;
   const int first = fb.pos0 + w0 / a.group, last = fb.pos0 + (min(w0 + 32, fb.r_end) - 1) / a.group;  // the wave's positions
   const ScoreRule rule = score_rule(a.rl);
-  const RowRule rr = row_rule(a.rl, b, row_in ? pos : -1);
+  const RowRule rr = row_rule(a.rl, b, row_in ? pos : -1, c1);
   const int prefix = a.rl.prefix ? a.rl.prefix[b] : 0;
   const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
   const int* docs = a.rl.docs ? a.rl.docs + b * a.rl.docs_stride : nullptr;
@@ -327,20 +412,19 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
   Tile tile;
   tile.load_q(row_in && pos >= 0 ? static_cast<const TI*>(a.q) + row * a.q_stride + head * kv.hd : nullptr, kv.hd, rule.mul);
   if (tid == 0) {
-    s_docs[0] = INT_MAX;
-    s_docs[1] = -1;
+    s_tags[0] = docs ? INT_MAX : 0;
+    s_tags[1] = docs ? -1 : 0;
   }
-  if (tid < PR_ROWS) s_bad[tid] = 0;
   __syncthreads();
-  if (docs && half == 0 && rr.pos >= 0) {  // the range of the rows' documents
-    atomicMin(&s_docs[0], rr.doc);
-    atomicMax(&s_docs[1], rr.doc);
+  if (docs && half == 0 && rr.span) {  // the range of the rows' documents
+    atomicMin(&s_tags[0], rr.tag);
+    atomicMax(&s_tags[1], rr.tag);
   }
 
   // a wave's rows in a page, and their offsets in 32 bits
   const bool whole_pages = kv.page_mask >= 15 && kv.pos_stride <= 1 << 24;
   tile.set_lanes(kv.hd, static_cast<uint32_t>(kv.pos_stride));
-  const bool all_rows = !__any(row_in && rr.pos < 0);  // none of no document or before the start
+  const bool all_rows = !__any(row_in && rr.span == 0);  // none that sees nothing
 
   float m = MAX_START, z = 0.0f;
   for (int seg = c0; seg < c1; seg += SEG) {
@@ -354,7 +438,7 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
       for (int i = wv; i < n_tiles; i += 4) {
         const int j = seg + i * KT + lane;
         const int d = lane < KT && j < seg_end ? docs[j] : -1;
-        if (__any(d >= s_docs[0] && d <= s_docs[1]) && lane == 0) atomicOr(&s_tiles, 1u << i);
+        if (__any(d >= s_tags[0] && d <= s_tags[1]) && lane == 0) atomicOr(&s_tiles, 1u << i);
       }
       __syncthreads();
     }
@@ -377,79 +461,97 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
       if (whole_pages && p0 + KT <= seg_end) tile.load_whole(kc, vc, p0, wv, kv.hd, kv.pos_stride, base);
       else tile.load(kc, vc, p0, kv.hd, offset);
     };
+    const bool tagged = docs || bad_pages;
+    auto stage_tags = [&](int at, int p0) {
+      if (!tagged || wv) return;
+      const int tag = lane < KT ? tag_of(a.rl, a.bt, kv, b, min(p0 + lane, seg_end - 1), bad_pages) : s_tags[0];
+      if (lane < KT) s_tag[at][lane] = tag;
+      const bool plain = !__any(tag != s_tags[0]);
+      if (lane == 0) s_plain[at] = plain;
+    };
+    // The rules on the scores of 32 positions, and the running maximum.  Returns what takes
+    // the scores to units of log2; `f` gets what the shares so far are multiplied by.
+    auto shape = [&](f32x16& s, int p0, int u, int at, float& f) {
+      const int pp = p0 + 32 * u;  // the lane: positions pp + 8 (i / 4) + 4 half + i % 4
+      // one tag in the tile and in the rows: nothing to tell apart
+      const bool tags = tagged && !(s_tags[0] == s_tags[1] && s_plain[at]);
+      const bool masked = tags || !all_rows || pp + 31 > first || pp + 32 > seg_end || (a.rl.window > 0 && last - pp >= a.rl.window);
+      float scale = tile.mul;
+      if (rule.capped || a.rl.slopes || masked || !(rule.mul > 0.0f)) {  // the same for the wave
+#pragma unroll
+        for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(s[i]));  // nothing of this ahead of the branch
+        scale = 1.0f;
+        scores_of<16>(rule, s, tile.mul);
+        if (a.rl.slopes) {
+          const float far = static_cast<float>(pos - (pp + 4 * half));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope, fabsf(far - static_cast<float>(8 * (i / 4) + i % 4)), s[i]);
+        }
+        if (masked) {
+          const int j0 = pp + 4 * half - rr.lo;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[i] = static_cast<unsigned>(j0 + 8 * (i / 4) + i % 4) < rr.span ? s[i] : -__builtin_inff();
+          if (tags) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = s_tag[at][32 * u + 8 * (i / 4) + 4 * half + i % 4] == rr.tag ? s[i] : -__builtin_inff();
+          }
+        }
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top = __builtin_fmaf(top, scale, -LIFT);
+      f = 1.0f;
+      if (__any(top > m + SLACK)) {
+        top = fmaxf(top, lane_xor32(top));
+        const float mn = fmaxf(m, top);
+        f = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        z *= f;
+#pragma unroll
+        for (int j = 0; j < Tile::NO; ++j) tile.o[j] *= f;
+      }
+      return scale;
+    };
     int cur = __builtin_ctz(todo), buf = 0;
     todo &= todo - 1;
     load(seg + cur * KT);
     tile.store(s_tile[0]);
-    auto stage_docs = [&](int at, int p0) {
-      if (!docs || wv) return;
-      const int d = lane < KT ? docs[min(p0 + lane, seg_end - 1)] : s_docs[0];
-      if (lane < KT) s_doc[at][lane] = d;
-      const bool plain = !__any(d != s_docs[0]);
-      if (lane == 0) s_plain[at] = plain;
-    };
-    stage_docs(0, seg + cur * KT);
+    stage_tags(0, seg + cur * KT);
     for (;;) {
       const int next = todo ? __builtin_ctz(todo) : -1;
       todo &= todo - 1;
       __syncthreads();
       if (next >= 0) load(seg + next * KT);
       const int p0 = seg + cur * KT;
-      // one document in the tile and in the rows: nothing to tell apart
-      const bool doc_masks = docs && !(s_docs[0] == s_docs[1] && s_plain[buf]);
       if (wave_in && (p0 <= last || p0 < prefix) && !(a.rl.window > 0 && first - (p0 + KT - 1) >= a.rl.window)) {
+        f32x16 s0;
+        float p[16], f;
+        if constexpr (KT == 64) {
+          f32x16 s1;
+          float p1[16];
+          const char *k0 = tile.k_at(s_tile[buf], 0), *k1 = tile.k_at(s_tile[buf], 1), *v0 = tile.v_at(s_tile[buf], 0), *v1 = tile.v_at(s_tile[buf], 1);
+          tile.begin_k(k0);
+          tile.scores(s0, k0);
+          tile.begin_k(k1);
+          float scale = shape(s0, p0, 0, buf, f);
+          tile.scores_and_shares(s1, k1, s0, p, scale, m, z, v0);
+          scale = shape(s1, p0, 1, buf, f);
+          if (__any(f != 1.0f)) {
 #pragma unroll
-        for (int sub = 0; sub < KT / 32; ++sub) {
-          const int pp = p0 + 32 * sub;  // the lane: positions pp + 8 (i / 4) + 4 half + i % 4
-          f32x16 s = tile.scores(s_tile[buf], sub);
-          const bool masked = doc_masks || !all_rows || bad_pages || pp + 31 > first || pp + 32 > seg_end || (a.rl.window > 0 && last - pp >= a.rl.window);
-          const bool shaped = rule.capped || a.rl.slopes || masked || !(rule.mul > 0.0f);  // the same for the wave
-          float scale = tile.mul;
-          if (shaped) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) asm volatile("" : "+v"(s[i]));  // nothing of this ahead of the branch
-            scale = 1.0f;
-            scores_of<16>(rule, s, tile.mul);
-            if (a.rl.slopes) {
-              const float far = static_cast<float>(pos - (pp + 4 * half));
-#pragma unroll
-              for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope, fabsf(far - static_cast<float>(8 * (i / 4) + i % 4)), s[i]);
-            }
-            if (masked) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int o = 32 * sub + 8 * (i / 4) + 4 * half + i % 4, j = p0 + o;
-                bool ok = (j < seg_end) & ((j <= rr.pos) | (j < rr.prefix)) & (rr.pos - j < rr.window);
-                if (docs) ok &= s_doc[buf][o] == rr.doc;
-                if (bad_pages) ok &= page_of(a.bt, kv, b, min(j, seg_end - 1)) >= 0;
-                s[i] = ok ? s[i] : -__builtin_inff();
-              }
-            }
+            for (int i = 0; i < 16; ++i) p[i] *= f;
           }
-          float top = s[0];
-#pragma unroll
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-          top = __builtin_fmaf(top, scale, -LIFT);
-          if (__any(top > m + SLACK)) {
-            top = fmaxf(top, lane_xor32(top));
-            const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            z *= f;
-#pragma unroll
-            for (int j = 0; j < Tile::NO; ++j) tile.o[j] *= f;
-          }
-          float p[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -m));
-            z += p[i];
-          }
-          tile.add(s_tile[buf], sub, p);
+          tile.template outputs<true>(p, v0, s1, p1, scale, m, z, v1);
+          tile.template outputs<false>(p1, v1, s1, p, scale, m, z, v1);
+        } else {
+          tile.scores(s0, s_tile[buf]);
+          const float scale = shape(s0, p0, 0, buf, f);
+          tile.step(s0, scale, m, z, s_tile[buf]);
         }
       }
       if (next < 0) break;
       tile.store(s_tile[buf ^ 1]);
-      stage_docs(buf ^ 1, seg + next * KT);
+      stage_tags(buf ^ 1, seg + next * KT);
       cur = next;
       buf ^= 1;
     }
@@ -459,8 +561,9 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
   const bool final = a.n_splits == 1;
   const float inv = z == 0.0f ? 0.0f : 1.0f / z;
   const int64_t at = part_index(a, b, t, head, split);
+  bool bad = false;
   if (row_in) {
-    bool bad = !(z < __builtin_inff());
+    bad = !(z < __builtin_inff());
     TI* dst = static_cast<TI*>(a.out) + row * a.out_stride + head * kv.hd;
     float* part = a.part_o + at * kv.hd;
 #pragma unroll
@@ -474,29 +577,29 @@ __global__ void __launch_bounds__(256, DP <= 128 ? 2 : 1) k_attention_prompt(con
           bad = bad || x[i] - x[i] != 0.0f;
         }
 #pragma unroll
-        for (int i = 0; i < Tile::RUN; ++i)
-          if (final) dst[d + i] = static_cast<TI>(x[i] * inv);
-          else part[d + i] = x[i];
+        for (int i = 0; i < Tile::RUN; ++i) x[i] = final ? x[i] * inv : x[i];
+        if (final) {
+          typedef TI Out __attribute__((ext_vector_type(Tile::RUN)));
+          Out y;
+#pragma unroll
+          for (int i = 0; i < Tile::RUN; ++i) y[i] = static_cast<TI>(x[i]);
+          *reinterpret_cast<Out*>(dst + d) = y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < Tile::RUN; i += 2) *reinterpret_cast<float2*>(part + d + i) = make_float2(x[i], x[i + 1]);
+        }
       }
     }
     if (half == 0 && a.part_mz) a.part_mz[at] = make_float2(m, z);
-    if (bad) s_bad[r - rb * PR_ROWS] = 1;
   }
-  __syncthreads();
+  if (!__syncthreads_or(bad)) return;
   // Something infinite or NaN came up: perhaps only a share of 0 times it.
+  if (tid < PR_ROWS) s_bad[tid] = 0;
+  __syncthreads();
+  if (bad) s_bad[r - rb * PR_ROWS] = 1;
+  __syncthreads();
   float* lds = reinterpret_cast<float*>(s_tile[0]);
-  for (int i = 0; i < PR_ROWS && rb * PR_ROWS + i < fb.r_end; ++i) {
-    if (!s_bad[i]) continue;
-    const int ri = rb * PR_ROWS + i, ti = ri / a.group, hi = kh * a.group + ri - ti * a.group;
-    float2 mz;
-    const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + ti, hi, fb.pos0 + ti, c0, c1, lds, lds + PAGED_MAX_HD, lds + 2 * PAGED_MAX_HD, &mz);
-    const int64_t ai = part_index(a, b, ti, hi, split);
-    if (tid < kv.hd) {
-      if (final) static_cast<TI*>(a.out)[(sr.r0 + ti) * a.out_stride + hi * kv.hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
-      else a.part_o[ai * kv.hd + tid] = o;
-    }
-    if (tid == 0 && a.part_mz) a.part_mz[ai] = mz;
-  }
+  exact_rows<TC, TI>(b, kh, rb, split, PR_ROWS, s_bad, lds, lds + PAGED_MAX_HD, lds + 2 * PAGED_MAX_HD);
 }
 
 template <typename TC, typename TI, int DP>

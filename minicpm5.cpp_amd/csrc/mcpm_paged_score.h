@@ -109,25 +109,28 @@ __device__ __forceinline__ void scores_of(const ScoreRule& sr, Dots& s, float mu
   }
 }
 
-// A row's place under the rules; pos < 0 (no row, or one of no document) sees nothing.
+// What a row sees: the positions j with 0 <= j - lo < span whose tag is the row's.  A
+// position's tag is its document, 0 without documents; HIDDEN_TAG where its page is
+// outside the pool.
+constexpr int HIDDEN_TAG = -2;
 struct RowRule {
-  int pos, prefix, window, doc;
+  int lo;
+  unsigned span;
+  int tag;
 };
-__device__ __forceinline__ RowRule row_rule(const RuleView& rl, int b, int pos) {
-  RowRule r{pos, rl.prefix ? rl.prefix[b] : 0, rl.window > 0 ? rl.window : 0x7fffffff, 0};
-  if (rl.docs && pos >= 0) {
-    r.doc = rl.docs[b * rl.docs_stride + pos];
-    if (r.doc < 0) r.pos = -1;
-  }
-  if (r.pos < 0) r.prefix = 0;
-  return r;
+// pos < 0 (no row, or one before the start) sees nothing, as does a row of no document.
+__device__ __forceinline__ RowRule row_rule(const RuleView& rl, int b, int pos, int end) {
+  if (pos < 0) return RowRule{0, 0, 0};
+  const int tag = rl.docs ? rl.docs[b * rl.docs_stride + pos] : 0;
+  const int hi = min(max(pos + 1, rl.prefix ? rl.prefix[b] : 0), end);
+  const int lo = rl.window > 0 ? max(pos - rl.window + 1, 0) : 0;
+  return RowRule{lo, tag < 0 || hi <= lo ? 0u : static_cast<unsigned>(hi - lo), tag};
 }
-// Whether the row sees position j, 0 <= j < the sequence's length.
-__device__ __forceinline__ bool seen(const RuleView& rl, const RowRule& r, int b, int j) {
-  bool ok = (j <= r.pos) | (j < r.prefix);
-  ok &= r.pos - j < r.window;
-  if (rl.docs) ok &= rl.docs[b * rl.docs_stride + j] == r.doc;
-  return ok;
+__device__ __forceinline__ bool in_span(const RowRule& r, int j) { return static_cast<unsigned>(j - r.lo) < r.span; }
+// The tag of position j, which has to be below the sequence's length.
+__device__ __forceinline__ int tag_of(const RuleView& rl, const BatchView& bt, const PagedView& kv, int b, int j, bool bad_pages) {
+  const int tag = rl.docs ? rl.docs[b * rl.docs_stride + j] : 0;
+  return bad_pages && page_of(bt, kv, b, j) < 0 ? HIDDEN_TAG : tag;
 }
 
 // Positions [lo, hi) that rows at pos0 .. pos1 may see, lo at a multiple of 64.
@@ -192,6 +195,14 @@ __device__ __forceinline__ bool load_page_offsets(const BatchView& bt, const Pag
   return ok;
 }
 
+// The call's own copy in the kernel's arguments: what the rare ends of a kernel need
+// is read again there rather than held in scalar registers through its loops.
+__device__ __forceinline__ const PagedCall& call_again() {
+  const void* p = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *static_cast<const PagedCall*>(p);
+}
+
 // The plain computation of one row over positions [c0, c1), by the whole work
 // group, for values that the matrix products cannot keep apart: a share of 0
 // times what a masked place holds.  Returns this lane's element tid of sum
@@ -205,13 +216,13 @@ __device__ __forceinline__ float exact_row(const PagedCall& a, int b, int kh, in
   if (tid < hd) s_q[tid] = static_cast<float>(static_cast<const TI*>(a.q)[row * a.q_stride + head * hd + tid]);
   __syncthreads();
   const ScoreRule sr = score_rule(a.rl);
-  const RowRule rr = row_rule(a.rl, b, pos);
+  const RowRule rr = row_rule(a.rl, b, pos, c1);
   const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
   float m = MAX_START, z = 0.0f, o = 0.0f;
   for (int j0 = c0; j0 < c1; j0 += 256) {
     const int j = j0 + tid;
     float s = -__builtin_inff();
-    const int page = j < c1 && pos >= 0 && seen(a.rl, rr, b, j) ? page_of(a.bt, kv, b, j) : -1;
+    const int page = in_span(rr, j) && tag_of(a.rl, a.bt, kv, b, j, false) == rr.tag ? page_of(a.bt, kv, b, j) : -1;
     if (page >= 0) {
       const TC* k = reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh);
       float d = 0.0f;
@@ -241,6 +252,30 @@ __device__ __forceinline__ float exact_row(const PagedCall& a, int b, int kh, in
   }
   *mz = make_float2(m, z);
   return o;
+}
+
+// exact_row for the rows of a block (those that `bad` marks, all without it), stored as
+// the block's own were.  Chunk `split` of the block's positions.
+template <typename TC, typename TI>
+__device__ __forceinline__ void exact_rows(int b, int kh, int rb, int split, int rows, const unsigned char* bad, float* s_q, float* s_p, float* s_red) {
+  const PagedCall& a = call_again();
+  const int tid = threadIdx.x, hd = a.kv.hd;
+  const SeqRows sr = seq_rows(a.bt, b);
+  const RowBlock blk = row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b));
+  const int c0 = blk.keys.lo + split * a.chunk, c1 = min(blk.keys.hi, c0 + a.chunk);
+#pragma unroll 1
+  for (int i = 0; i < rows && rb * rows + i < blk.r_end; ++i) {
+    if (bad && !bad[i]) continue;
+    const int r = rb * rows + i, t = r / a.group, head = kh * a.group + r - t * a.group;
+    float2 mz;
+    const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + t, head, blk.pos0 + t, c0, c1, s_q, s_p, s_red, &mz);
+    const int64_t at = part_index(a, b, t, head, split);
+    if (tid < hd) {
+      if (a.n_splits == 1) static_cast<TI*>(a.out)[(sr.r0 + t) * a.out_stride + head * hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
+      else a.part_o[at * hd + tid] = o;
+    }
+    if (tid == 0 && a.part_mz) a.part_mz[at] = mz;
+  }
 }
 
 // The prompt kernels (mcpm_paged_prompt.hip): row blocks of prompt_block_rows rows.
