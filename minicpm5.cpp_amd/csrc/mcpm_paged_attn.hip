@@ -5,6 +5,7 @@
 //
 // Scores are held in units of log2.
 #include <algorithm>
+#include <climits>
 
 #include "mcpm_paged_score.h"
 
@@ -28,12 +29,11 @@ namespace {
 constexpr int FEW_ROWS = 16;
 constexpr int FEW_STEP = 32;                // positions of a wave's step
 constexpr int FEW_ROUND = 4 * FEW_STEP;     // of a work group's
-constexpr int FEW_MIN_CHUNK = 256;
-constexpr int FEW_TARGET = 4;               // work groups per CU
+constexpr int FEW_MAX_ROUNDS = 16;          // rounds of a work group, at most: its table of pages is in LDS
+constexpr int FEW_TARGET = 1, FEW_TARGET_64 = 4;  // work groups per CU that the work is shared among; heads of up to 64
 constexpr int PROMPT_TARGET = 1;            // work groups per CU that a prompt's length is split for
 constexpr int PROMPT_MIN_CHUNK = 512;
 constexpr int FEW_MOST = 32;                // new tokens x group up to which these kernels run
-constexpr int FEW_MAX_CHUNK = 2048;         // positions of a work group, at most
 
 template <typename TC, typename TI, int DP>
 struct FewTile;
@@ -200,6 +200,74 @@ struct FewTile<float, float, DP> {
   }
 };
 
+// A sequence's part of the work: rounds of positions that its rows may see, row blocks.
+struct SeqWork {
+  KeyRange keys;
+  int rounds, blocks;
+};
+__device__ __forceinline__ SeqWork seq_work(const PagedCall& a, int b) {
+  const SeqRows sr = seq_rows(a.bt, b);
+  if (!sr.n) return SeqWork{{0, 0}, 0, 0};
+  const int len = seq_len(a.bt, a.kv, b), pos0 = len - sr.given;
+  const KeyRange k = key_range(a.rl, b, pos0, pos0 + sr.n - 1, len);
+  return SeqWork{k, k.hi > k.lo ? (k.hi - k.lo + FEW_ROUND - 1) / FEW_ROUND : 1, (sr.n * a.group + FEW_ROWS - 1) / FEW_ROWS};
+}
+
+// Which part of which sequence this work group has.  The host knows a bound of the
+// lengths only, and they are ragged: every work group sums up the rounds of all
+// sequences and takes its share of them, the same number of rounds (the last of a
+// sequence fewer).  A block's chunks are `stride` work groups apart.
+struct Share {
+  int b, chunk, n_chunks, kh, rb, rounds, first;
+};
+__device__ __forceinline__ bool few_share(const PagedCall& a, Share* s_share, int64_t (*s_wave)[4], Share& out) {
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = a.kv.n_kv_heads, n = a.bt.n_seq;
+  SeqWork w = seq_work(a, min(tid, n - 1));
+  int64_t sum = 0;
+  for (int b = tid; b < n; b += 256) {
+    const SeqWork x = b == tid ? w : seq_work(a, b);
+    sum += static_cast<int64_t>(x.rounds) * x.blocks * per;
+  }
+  for (int s = 32; s; s >>= 1) sum += __shfl_xor(sum, s);
+  if (lane == 0) s_wave[0][wv] = sum;
+  if (tid == 0) s_share->b = -1;
+  __syncthreads();
+  const int64_t total = s_wave[0][0] + s_wave[0][1] + s_wave[0][2] + s_wave[0][3];
+  const int rounds = static_cast<int>(min(max((total + a.chunk - 1) / a.chunk, static_cast<int64_t>(1)), static_cast<int64_t>(FEW_MAX_ROUNDS)));
+  int64_t base = 0;
+  for (int b0 = 0; b0 < n; b0 += 256) {
+    const int b = b0 + tid;
+    if (b0 && b < n) w = seq_work(a, b);
+    const int chunks = b < n ? (w.rounds + rounds - 1) / rounds : 0;
+    const int64_t mine = static_cast<int64_t>(chunks) * w.blocks * per;
+    int64_t x = mine;
+    for (int s = 1; s < 64; s <<= 1) {
+      const int64_t y = __shfl_up(x, s);
+      x += lane >= s ? y : 0;
+    }
+    __syncthreads();
+    if (lane == 63) s_wave[1][wv] = x;
+    __syncthreads();
+    for (int i = 0; i < 4; ++i) x += i < wv ? s_wave[1][i] : 0;
+    const int64_t first = base + x - mine, i = static_cast<int64_t>(blockIdx.x) - first;
+    if (i >= 0 && i < mine) {
+      const int k = static_cast<int>(i), pairs = w.blocks * per;
+      *s_share = Share{b, k / pairs, chunks, k % per, k % pairs / per, rounds, static_cast<int>(first)};
+    }
+    base += s_wave[1][0] + s_wave[1][1] + s_wave[1][2] + s_wave[1][3];
+  }
+  __syncthreads();
+  out = *s_share;
+  out.b = __builtin_amdgcn_readfirstlane(out.b);
+  out.chunk = __builtin_amdgcn_readfirstlane(out.chunk);
+  out.n_chunks = __builtin_amdgcn_readfirstlane(out.n_chunks);
+  out.kh = __builtin_amdgcn_readfirstlane(out.kh);
+  out.rb = __builtin_amdgcn_readfirstlane(out.rb);
+  out.rounds = __builtin_amdgcn_readfirstlane(out.rounds);
+  out.first = __builtin_amdgcn_readfirstlane(out.first);
+  return out.b >= 0;
+}
+
 template <typename TC, typename TI, int DP>
 __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   __shared__ __attribute__((aligned(16))) float s_o[4][FEW_ROWS][DP + 4];
@@ -208,15 +276,18 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   extern __shared__ int64_t s_off[];
   const PagedView& kv = a.kv;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, n16 = lane & 15, g = lane >> 4;
-  const int b = blockIdx.y;
-  const int per = kv.n_kv_heads * a.n_blocks;
-  const int split = blockIdx.x / per, kh = blockIdx.x % per % kv.n_kv_heads, rb = blockIdx.x % per / kv.n_kv_heads;
+  __shared__ Share s_share;
+  __shared__ int64_t s_sum[2][4];
+  Share sh;
+  if (!few_share(a, &s_share, s_sum, sh)) return;
+  const int b = sh.b, kh = sh.kh, rb = sh.rb;
   const SeqRows sr = seq_rows(a.bt, b);
   const int len = seq_len(a.bt, kv, b);
-  if (rb * FEW_ROWS >= sr.n * a.group) return;
   const RowBlock fb = row_block(a, b, rb, sr, len);
-  const int c0 = fb.keys.lo + split * a.chunk, c1 = min(fb.keys.hi, c0 + a.chunk);
-  if (split && c0 >= fb.keys.hi) return;  // the first one answers for rows that see nothing
+  const KeyRange keys = key_range(a.rl, b, fb.pos0, fb.pos0 + sr.n - 1, len);
+  const int c0 = keys.lo + sh.chunk * sh.rounds * FEW_ROUND, c1 = min(keys.hi, c0 + sh.rounds * FEW_ROUND);
+  const bool final = sh.n_chunks == 1;
+  if (static_cast<int>(blockIdx.x) == sh.first && tid == 0 && a.seq_wgs) a.seq_wgs[b] = make_int2(sh.first, sh.n_chunks);
 
   const int r = rb * FEW_ROWS + n16;
   const bool row_in = r < fb.r_end;
@@ -331,8 +402,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
     Z += w[i] * s_z[i][rn];
   }
   const int64_t rowj = sr.r0 + tj;
-  const int64_t at = part_index(a, b, tj, hj, split);
-  const bool final = a.n_splits == 1;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * FEW_ROWS + rn;
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
   TI* dst = static_cast<TI*>(a.out) + rowj * a.out_stride + hj * kv.hd;
   bool bad = !(Z < __builtin_inff());
@@ -353,93 +423,143 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
       }
     }
   }
-  if (in && part == 0 && a.part_mz) a.part_mz[at] = make_float2(M, Z);
+  if (in && part == 0) {
+    if (a.part_mz) a.part_mz[at] = make_float2(M, Z);
+    if (final && a.row_mz) a.row_mz[row_index(a, b, tj, hj)] = make_float2(M, Z);
+  }
   if (in && bad) s_bad = 1;
   __syncthreads();
   if (!s_bad) return;
   // Something infinite or NaN came up: perhaps only a share of 0 times it.
-  exact_rows<TC, TI>(b, kh, rb, split, FEW_ROWS, nullptr, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0]);
+  exact_rows<TC, TI>(b, kh, rb, FEW_ROWS, c0, c1, final, nullptr, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0],
+                     [](const PagedCall&, int i, int, int) { return static_cast<int64_t>(blockIdx.x) * FEW_ROWS + i; });
 }
 
-__device__ __forceinline__ int active_splits(const PagedCall& a, const KeyRange& k) {
-  return k.hi > k.lo ? (k.hi - k.lo + a.chunk - 1) / a.chunk : 1;
+// Where a row's partials are: n of them, `stride` apart.
+struct Parts {
+  int64_t at, stride;
+  int n;
+};
+template <bool FEW>
+__device__ __forceinline__ Parts parts_of(const PagedCall& a, int b, const SeqRows& sr, int t, int head) {
+  const int r = t * a.group + head % a.group, rb = r / a.block_rows;
+  if constexpr (FEW) {
+    const int2 w = a.seq_wgs[b];
+    const int blocks = (sr.n * a.group + FEW_ROWS - 1) / FEW_ROWS, per = a.kv.n_kv_heads;
+    return Parts{(static_cast<int64_t>(w.x) + rb * per + head / a.group) * FEW_ROWS + r % FEW_ROWS, static_cast<int64_t>(blocks) * per * FEW_ROWS, w.y};
+  } else {
+    const KeyRange k = row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b)).keys;
+    return Parts{part_index(a, b, t, head, 0), 1, k.hi > k.lo ? (k.hi - k.lo + a.chunk - 1) / a.chunk : 1};
+  }
+}
+// (m, z) x joined to mz; returns what the two are multiplied by.
+__device__ __forceinline__ float2 join_mz(float2& mz, const float2& x) {
+  const float m = fmaxf(mz.x, x.x), f = __builtin_amdgcn_exp2f(mz.x - m), w = __builtin_amdgcn_exp2f(x.x - m);
+  mz = make_float2(m, f * mz.y + w * x.y);
+  return make_float2(f, w);
 }
 
-// The splits' partials of ROWS (new token, head)s into the output, a work group:
-// DP/4 lanes hold a row's elements, 256 / (DP/4) / ROWS of them take its splits in turn.
-template <typename TI, int DP, int ROWS>
-__global__ void __launch_bounds__(256) k_attention_join(const PagedCall a) {
+// The partials of ROWS (new token, head)s into the output, a work group: DP/4 lanes hold
+// a row's elements, 256 / (DP/4) / ROWS of them take its partials in turn.
+template <bool FEW, typename TI, int DP, int ROWS>
+__device__ __forceinline__ void join_rows(const PagedCall& a, int block, int b, char* lds) {
   constexpr int LP = DP / 4, GR = 256 / LP / ROWS;
-  __shared__ f32x4 s_acc[ROWS][GR][LP];
-  __shared__ float2 s_mz[ROWS][GR];
-  const int b = blockIdx.y, tid = threadIdx.x, hd = a.kv.hd;
+  f32x4* s_acc = reinterpret_cast<f32x4*>(lds);                       // [ROWS][GR][LP]
+  float2* s_mz = reinterpret_cast<float2*>(lds + 256 * sizeof(f32x4));  // [ROWS][GR]
+  const int tid = threadIdx.x, hd = a.kv.hd;
   const int e = tid % LP, g = tid / LP % GR, i = tid / LP / GR;
   const SeqRows sr = seq_rows(a.bt, b);
-  const int item = blockIdx.x * ROWS + i, t = item / a.n_heads, head = item - t * a.n_heads;
+  const int item = block * ROWS + i, t = item / a.n_heads, head = item - t * a.n_heads;
   const bool in = t < sr.n;
   f32x4 acc{0, 0, 0, 0};
   float2 mz = make_float2(MAX_START, 0.0f);
-  int64_t at = 0;
+  bool done = !in;
   if (in) {
-    const int rb = (t * a.group + head % a.group) / a.block_rows;
-    const int n = active_splits(a, row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b)).keys);
-    at = part_index(a, b, t, head, 0);
-    for (int k = g; k < n; k += GR) {
-      const float2 x = a.part_mz[at + k];
+    const Parts p = parts_of<FEW>(a, b, sr, t, head);
+    done = FEW && p.n == 1;  // the work group that had the row stored it
+    for (int k = g; k < p.n && !done; k += GR) {
+      const int64_t at = p.at + k * p.stride;
+      const float2 x = a.part_mz[at];
       if (x.y == 0.0f) continue;
-      const f32x4 o = e * 4 < hd ? *reinterpret_cast<const f32x4*>(a.part_o + (at + k) * hd + e * 4) : f32x4{0, 0, 0, 0};
-      const float m = fmaxf(mz.x, x.x), f = __builtin_amdgcn_exp2f(mz.x - m), w = __builtin_amdgcn_exp2f(x.x - m);
-      acc = f * acc + w * o;
-      mz = make_float2(m, f * mz.y + w * x.y);
+      const f32x4 o = e * 4 < hd ? *reinterpret_cast<const f32x4*>(a.part_o + at * hd + e * 4) : f32x4{0, 0, 0, 0};
+      const float2 f = join_mz(mz, x);
+      acc = f.x * acc + f.y * o;
     }
   }
   if constexpr (GR > 1) {
-    s_acc[i][g][e] = acc;
-    if (e == 0) s_mz[i][g] = mz;
+    s_acc[(i * GR + g) * LP + e] = acc;
+    if (e == 0) s_mz[i * GR + g] = mz;
     __syncthreads();
     if (g) return;
     for (int k = 1; k < GR; ++k) {
-      const float2 x = s_mz[i][k];
-      const float m = fmaxf(mz.x, x.x), f = __builtin_amdgcn_exp2f(mz.x - m), w = __builtin_amdgcn_exp2f(x.x - m);
-      acc = f * acc + w * s_acc[i][k][e];
-      mz = make_float2(m, f * mz.y + w * x.y);
+      const float2 f = join_mz(mz, s_mz[i * GR + k]);
+      acc = f.x * acc + f.y * s_acc[(i * GR + k) * LP + e];
     }
   }
-  if (!in) return;
-  if (e == 0 && a.kv.weight) a.part_mz[at] = mz;
+  if (done) return;
+  if (e == 0 && a.row_mz) a.row_mz[row_index(a, b, t, head)] = mz;
   if (e * 4 >= hd) return;
   const float inv = mz.y == 0.0f ? 0.0f : 1.0f / mz.y;
   TI* dst = static_cast<TI*>(a.out) + (sr.r0 + t) * a.out_stride + head * hd + e * 4;
 #pragma unroll
   for (int k = 0; k < 4; ++k) dst[k] = static_cast<TI>(acc[k] * inv);
 }
+constexpr int JOIN_LDS = 256 * (sizeof(f32x4) + sizeof(float2));
 
-// The positions' weights from the scores: a lane per position sums its rows in order.
-__global__ void __launch_bounds__(256) k_attention_weight(const PagedCall a) {
-  __shared__ float2 s_mz[FEW_ROWS];
-  const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, j = blockIdx.x * 256 + tid;
+template <typename TI, int DP, int ROWS>
+__global__ void __launch_bounds__(256) k_attention_join(const PagedCall a) {
+  __shared__ __attribute__((aligned(16))) char lds[JOIN_LDS];
+  join_rows<false, TI, DP, ROWS>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// The weights of 1024 positions of a kv head from the scores: a lane has four, and sums
+// the rows in order.  The rows' (m, z) are joined from the partials here too, so that
+// this runs beside the join.
+__device__ __forceinline__ void add_weights(const PagedCall& a, int kh, int chunk, int b, char* lds) {
+  float2* s_mz = reinterpret_cast<float2*>(lds);
+  const int tid = threadIdx.x, j = chunk * 1024 + tid * 4;
   const int len = seq_len(a.bt, a.kv, b);
-  if (static_cast<int>(blockIdx.x) * 256 >= len) return;
+  if (chunk * 1024 >= len) return;
   const SeqRows sr = seq_rows(a.bt, b);
+  const SeqWork w = seq_work(a, b);
   const int rows = sr.n * a.group;
   const float* sc = a.scores + (static_cast<int64_t>(b) * a.kv.n_kv_heads + kh) * a.score_rows * a.score_len + j;
-  float sum = 0.0f;
+  f32x4 sum{0, 0, 0, 0};
   for (int r0 = 0; r0 < rows; r0 += FEW_ROWS) {
-    const RowBlock fb = row_block(a, b, r0 / FEW_ROWS, sr, len);
     __syncthreads();
     if (tid < FEW_ROWS && r0 + tid < rows) {
       const int t = (r0 + tid) / a.group;
-      const float2 mz = a.part_mz[part_index(a, b, t, kh * a.group + r0 + tid - t * a.group, 0)];
+      const Parts p = parts_of<true>(a, b, sr, t, kh * a.group + r0 + tid - t * a.group);
+      float2 mz = make_float2(MAX_START, 0.0f);
+      for (int k = 0; k < p.n; ++k) join_mz(mz, a.part_mz[p.at + k * p.stride]);
       s_mz[tid] = make_float2(mz.x, mz.y == 0.0f ? 0.0f : 1.0f / mz.y);
     }
     __syncthreads();
-    if (j >= fb.keys.lo && j < fb.keys.hi)
-      for (int i = 0; i < FEW_ROWS && r0 + i < rows; ++i)
-        sum += __builtin_amdgcn_exp2f(sc[static_cast<int64_t>(r0 + i) * a.score_len] - s_mz[i].x) * s_mz[i].y;
+    if (j < w.keys.hi)
+      for (int i = 0; i < FEW_ROWS && r0 + i < rows; ++i) {
+        const f32x4 s = *reinterpret_cast<const f32x4*>(sc + static_cast<int64_t>(r0 + i) * a.score_len);
+        const float2 mz = s_mz[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (j + k >= w.keys.lo && j + k < w.keys.hi) sum[k] += __builtin_amdgcn_exp2f(s[k] - mz.x) * mz.y;
+      }
   }
-  if (j >= len) return;
-  const int page = page_of(a.bt, a.kv, b, j);
-  if (page >= 0) *weight_of(a.kv, page, j, kh) += sum;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (j + k >= w.keys.hi) break;
+    const int page = page_of(a.bt, a.kv, b, j + k);
+    if (page >= 0) *weight_of(a.kv, page, j + k, kh) += sum[k];
+  }
+}
+
+// After the few-row kernel, in one launch: `join_blocks` work groups a sequence join its
+// rows, the others add up the weights.
+template <typename TI, int DP, int ROWS>
+__global__ void __launch_bounds__(256) k_few_finish(const PagedCall a, int join_blocks) {
+  __shared__ __attribute__((aligned(16))) char lds[JOIN_LDS];
+  const int x = blockIdx.x, b = blockIdx.y;
+  if (x < join_blocks) join_rows<true, TI, DP, ROWS>(a, x, b, lds);
+  else add_weights(a, (x - join_blocks) % a.kv.n_kv_heads, (x - join_blocks) / a.kv.n_kv_heads, b, lds);
 }
 
 __device__ __forceinline__ float simple_score(const RuleView& rl, float slope, float dot, int pos, int j) {
@@ -467,7 +587,7 @@ __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
       const TI* q = static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + h * hd;
       float d = 0.0f;
       for (int i = 0; i < hd; ++i) d = __builtin_fmaf(static_cast<float>(q[i]), static_cast<float>(k[i]), d);
-      const float2 r = a.part_mz[part_index(a, b, t, h, 0)];
+      const float2 r = a.row_mz[row_index(a, b, t, h)];
       if (r.y != 0.0f) sum += __builtin_amdgcn_exp2f(simple_score(a.rl, a.rl.slopes ? a.rl.slopes[h] : 0.0f, d, pos, j) - r.x) / r.y;
     }
   }
@@ -478,10 +598,12 @@ __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
 // head take the 16-row kernel, more the prompt kernel.
 struct Plan {
   bool few;
-  int block_rows, n_blocks, chunk, n_splits, score_len;
-  size_t o_bytes, mz_bytes, score_bytes;
-  size_t bytes() const { return o_bytes + mz_bytes + score_bytes; }
+  int block_rows, n_blocks, chunk, n_splits, grid, score_len;
+  size_t o_bytes, mz_bytes, row_bytes, seq_bytes, score_bytes;
+  size_t bytes() const { return o_bytes + mz_bytes + row_bytes + seq_bytes + score_bytes; }
 };
+size_t round16(size_t n) { return (n + 15) / 16 * 16; }
+constexpr size_t MOST_SCORES = size_t{1} << 30;  // bytes of kept scores, past which they are formed again
 
 Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu) {
   Plan p{};
@@ -494,55 +616,78 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
   int64_t span = std::min<int64_t>(bt.max_len, table);
   p.score_len = static_cast<int>((span + 63) / 64 * 64);
   // rows of a block are at most block_rows positions apart, lo goes down to a multiple of 64
-  if (rl.window > 0 && !rl.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(rl.window) + p.block_rows + 64);
+  if (rl.window > 0 && !rl.prefix) span = std::min<int64_t>(span, static_cast<int64_t>(rl.window) + std::max(p.block_rows, FEW_MOST) + 64);
   span = std::max<int64_t>(span, 1);
   const int64_t blocks = static_cast<int64_t>(bt.n_seq) * kv.n_kv_heads * p.n_blocks;
+  size_t parts;
   if (p.few) {
-    const int64_t chunk = (span * blocks / (FEW_TARGET * n_cu) + FEW_ROUND) / FEW_ROUND * FEW_ROUND;
-    p.chunk = static_cast<int>(std::min<int64_t>(std::max<int64_t>(chunk, FEW_MIN_CHUNK), FEW_MAX_CHUNK));
+    const int64_t rounds = (span + FEW_ROUND - 1) / FEW_ROUND;
+    const int per_cu = kv.hd <= 64 ? FEW_TARGET_64 : FEW_TARGET;
+    p.chunk = per_cu * n_cu;
+    // few_share gives a sequence a work group more than its share, at most, and none more than FEW_MAX_ROUNDS
+    const int64_t most = std::max<int64_t>(p.chunk, blocks * ((rounds + FEW_MAX_ROUNDS - 1) / FEW_MAX_ROUNDS)) + blocks;
+    const int64_t grid = std::min(most, blocks * rounds);
+    p.grid = grid > INT_MAX ? -1 : static_cast<int>(grid);
+    p.n_splits = rounds > 1 ? 2 : 1;
+    parts = static_cast<size_t>(grid) * FEW_ROWS;
+    p.seq_bytes = p.n_splits > 1 || kv.weight ? round16(bt.n_seq * sizeof(int2)) : 0;
   } else {
     const int64_t want = std::max<int64_t>(1, PROMPT_TARGET * n_cu / blocks);
     p.chunk = static_cast<int>((std::max<int64_t>((span + want - 1) / want, PROMPT_MIN_CHUNK) + 63) / 64 * 64);
+    p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
+    parts = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.n_splits;
   }
-  p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
-  const size_t parts = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.n_splits;
+  const size_t all_rows = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads;
   if (p.n_splits > 1) p.o_bytes = parts * kv.hd * sizeof(float);
-  if (p.n_splits > 1 || kv.weight) p.mz_bytes = (parts * sizeof(float2) + 15) / 16 * 16;
-  if (kv.weight && p.few) p.score_bytes = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.score_len * sizeof(float);
+  if (p.n_splits > 1 || (kv.weight && p.few)) p.mz_bytes = round16(parts * sizeof(float2));
+  if (kv.weight) {
+    p.score_bytes = p.few ? all_rows * p.score_len * sizeof(float) : 0;
+    if (p.score_bytes > MOST_SCORES) p.score_bytes = 0;
+    if (!p.score_bytes) p.row_bytes = round16(all_rows * sizeof(float2));
+  }
   return p;
 }
 
 template <typename TC, typename TI, int DP>
-hipError_t few(const PagedCall& a, hipStream_t s) {
-  const size_t lds = (static_cast<size_t>(a.chunk >> a.kv.page_shift) + 2) * sizeof(int64_t);
-  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(a.n_splits * a.kv.n_kv_heads * a.n_blocks, a.bt.n_seq), dim3(256), lds, s, a);
+hipError_t few(const PagedCall& a, int grid, hipStream_t s) {
+  const size_t lds = (static_cast<size_t>(FEW_MAX_ROUNDS * FEW_ROUND >> a.kv.page_shift) + 2) * sizeof(int64_t);
+  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(grid), dim3(256), lds, s, a);
   return hipGetLastError();
 }
 template <typename TC, typename TI>
-hipError_t few(const PagedCall& a, hipStream_t s) {
-  return a.kv.hd <= 64 ? few<TC, TI, 64>(a, s) : a.kv.hd <= 128 ? few<TC, TI, 128>(a, s) : few<TC, TI, 256>(a, s);
+hipError_t few(const PagedCall& a, int grid, hipStream_t s) {
+  return a.kv.hd <= 64 ? few<TC, TI, 64>(a, grid, s) : a.kv.hd <= 128 ? few<TC, TI, 128>(a, grid, s) : few<TC, TI, 256>(a, grid, s);
 }
-hipError_t launch_attention_few(const PagedCall& a, int kv_type, int io_type, hipStream_t s) {
+hipError_t launch_attention_few(const PagedCall& a, int grid, int kv_type, int io_type, hipStream_t s) {
+  if (grid < 0) return hipErrorInvalidValue;
   const bool f32 = io_type == MCPM_TYPE_F32;
-  if (kv_type == MCPM_TYPE_F32) return few<float, float>(a, s);
-  if (kv_type == MCPM_TYPE_F16) return f32 ? few<_Float16, float>(a, s) : few<_Float16, _Float16>(a, s);
-  return f32 ? few<__bf16, float>(a, s) : few<__bf16, __bf16>(a, s);
+  if (kv_type == MCPM_TYPE_F32) return few<float, float>(a, grid, s);
+  if (kv_type == MCPM_TYPE_F16) return f32 ? few<_Float16, float>(a, grid, s) : few<_Float16, _Float16>(a, grid, s);
+  return f32 ? few<__bf16, float>(a, grid, s) : few<__bf16, __bf16>(a, grid, s);
 }
 
+// What follows the main kernel: the join where rows are in parts, the weights' sum
+// where the scores were kept.
 template <typename TI, int DP>
-hipError_t join(const PagedCall& a, int n_cu, hipStream_t s) {
+hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
   constexpr int LP = DP / 4, MOST = 256 / LP;
-  const int items = a.bt.max_new * a.n_heads;
-  // rows side by side where that leaves a work group per CU, else the splits
-  if (static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu)
-    hipLaunchKernelGGL((k_attention_join<TI, DP, MOST>), dim3((items + MOST - 1) / MOST, a.bt.n_seq), dim3(256), 0, s, a);
-  else
-    hipLaunchKernelGGL((k_attention_join<TI, DP, 1>), dim3(items, a.bt.n_seq), dim3(256), 0, s, a);
+  const int items = a.bt.max_new * a.n_heads, groups = a.n_splits > 1 ? (items + MOST - 1) / MOST : 0;
+  // rows side by side where that leaves a work group per CU, else their partials
+  const bool side = static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu;
+  const int joins = a.n_splits == 1 ? 0 : side ? groups : items;
+  if (!few) {
+    if (side) hipLaunchKernelGGL((k_attention_join<TI, DP, MOST>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_attention_join<TI, DP, 1>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
+  } else {
+    const dim3 grid(joins + (a.scores ? (a.score_len + 1023) / 1024 * a.kv.n_kv_heads : 0), a.bt.n_seq);
+    if (side) hipLaunchKernelGGL((k_few_finish<TI, DP, MOST>), grid, dim3(256), 0, s, a, joins);
+    else hipLaunchKernelGGL((k_few_finish<TI, DP, 1>), grid, dim3(256), 0, s, a, joins);
+  }
   return hipGetLastError();
 }
 template <typename TI>
-hipError_t join(const PagedCall& a, int n_cu, hipStream_t s) {
-  return a.kv.hd <= 64 ? join<TI, 64>(a, n_cu, s) : a.kv.hd <= 128 ? join<TI, 128>(a, n_cu, s) : join<TI, 256>(a, n_cu, s);
+hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
+  return a.kv.hd <= 64 ? finish<TI, 64>(a, few, n_cu, s) : a.kv.hd <= 128 ? finish<TI, 128>(a, few, n_cu, s) : finish<TI, 256>(a, few, n_cu, s);
 }
 
 template <typename TC, typename TI>
@@ -563,20 +708,26 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
   const Plan p = plan_of(kv, bt, rl, n_heads, n_cu);
   const int group = n_heads / kv.n_kv_heads;
   char* sc = static_cast<char*>(scratch);
-  const PagedCall a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.block_rows, p.n_blocks, p.chunk, p.n_splits,
-                    reinterpret_cast<float*>(sc), p.mz_bytes ? reinterpret_cast<float2*>(sc + p.o_bytes) : nullptr,
-                    p.score_bytes ? reinterpret_cast<float*>(sc + p.o_bytes + p.mz_bytes) : nullptr, p.score_len, bt.max_new * group};
-  hipError_t e = p.few ? launch_attention_few(a, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
+  auto take = [&](size_t bytes) {
+    char* at = bytes ? sc : nullptr;
+    sc += bytes;
+    return at;
+  };
+  PagedCall a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.block_rows, p.n_blocks, p.chunk, p.n_splits};
+  a.part_o = reinterpret_cast<float*>(take(p.o_bytes));
+  a.part_mz = reinterpret_cast<float2*>(take(p.mz_bytes));
+  a.row_mz = reinterpret_cast<float2*>(take(p.row_bytes));
+  a.seq_wgs = reinterpret_cast<int2*>(take(p.seq_bytes));
+  a.scores = reinterpret_cast<float*>(take(p.score_bytes));
+  a.score_len = p.score_len;
+  a.score_rows = bt.max_new * group;
+  hipError_t e = p.few ? launch_attention_few(a, p.grid, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
   if (e != hipSuccess) return e;
-  if (p.n_splits > 1) {
-    e = io_type == MCPM_TYPE_F32 ? join<float>(a, n_cu, s) : io_type == MCPM_TYPE_F16 ? join<_Float16>(a, n_cu, s) : join<__bf16>(a, n_cu, s);
+  if (p.n_splits > 1 || a.scores) {
+    e = io_type == MCPM_TYPE_F32 ? finish<float>(a, p.few, n_cu, s) : io_type == MCPM_TYPE_F16 ? finish<_Float16>(a, p.few, n_cu, s) : finish<__bf16>(a, p.few, n_cu, s);
     if (e != hipSuccess) return e;
   }
-  if (!kv.weight || !p.score_len) return hipSuccess;
-  if (p.few) {
-    hipLaunchKernelGGL(k_attention_weight, dim3((p.score_len + 255) / 256, kv.n_kv_heads, bt.n_seq), dim3(256), 0, s, a);
-    return hipGetLastError();
-  }
+  if (!kv.weight || a.scores || !p.score_len) return hipSuccess;
   const bool f32 = io_type == MCPM_TYPE_F32;
   if (kv_type == MCPM_TYPE_F32) return prompt_weight<float, float>(a, s);
   if (kv_type == MCPM_TYPE_F16) return f32 ? prompt_weight<_Float16, float>(a, s) : prompt_weight<_Float16, _Float16>(a, s);

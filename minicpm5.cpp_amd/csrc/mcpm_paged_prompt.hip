@@ -590,7 +590,10 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
         }
       }
     }
-    if (half == 0 && a.part_mz) a.part_mz[at] = make_float2(m, z);
+    if (half == 0) {
+      if (a.part_mz) a.part_mz[at] = make_float2(m, z);
+      if (final && a.row_mz) a.row_mz[row_index(a, b, t, head)] = make_float2(m, z);
+    }
   }
   if (!__syncthreads_or(bad)) return;
   // Something infinite or NaN came up: perhaps only a share of 0 times it.
@@ -599,7 +602,8 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
   if (bad) s_bad[r - rb * PR_ROWS] = 1;
   __syncthreads();
   float* lds = reinterpret_cast<float*>(s_tile[0]);
-  exact_rows<TC, TI>(b, kh, rb, split, PR_ROWS, s_bad, lds, lds + PAGED_MAX_HD, lds + 2 * PAGED_MAX_HD);
+  exact_rows<TC, TI>(b, kh, rb, PR_ROWS, c0, c1, final, s_bad, lds, lds + PAGED_MAX_HD, lds + 2 * PAGED_MAX_HD,
+                     [&](const PagedCall& c, int, int tt, int h) { return part_index(c, b, tt, h, split); });
 }
 
 template <typename TC, typename TI, int DP>

@@ -147,8 +147,9 @@ __device__ __forceinline__ KeyRange key_range(const RuleView& rl, int b, int pos
 }
 
 // A call as its kernels see it.  A row block is `block_rows` rows of a sequence
-// (new tokens x the kv head's query heads, token by token); its positions are cut
-// into chunks of `chunk`, a work group each.
+// (new tokens x the kv head's query heads, token by token).  The prompt kernel cuts a
+// block's positions into chunks of `chunk`, a work group each; the few-row kernel
+// shares them out by the lengths that it finds (few_share).
 struct PagedCall {
   PagedView kv;
   BatchView bt;
@@ -157,15 +158,21 @@ struct PagedCall {
   void* out;
   int64_t q_stride, out_stride;
   int n_heads, group, block_rows, n_blocks;  // query heads per kv head; row blocks per (sequence, kv head)
-  int chunk, n_splits;
-  float* part_o;    // [seq][new token][head][split][hd], unnormalised
-  float2* part_mz;  // [seq][new token][head][split]; with weights, the first is the row's own at the end
-  float* scores;    // [seq][kv head][row of the sequence][score_len], or null
+  int chunk, n_splits;  // few rows: work groups wanted, and whether there can be more than one to a block
+  float* part_o;    // unnormalised: [seq][new token][head][split][hd]; few rows: [work group][row of the block][hd]
+  float2* part_mz;  // the same without [hd]
+  float2* row_mz;   // [seq][new token][head]: the rows' own, with weights
+  int2* seq_wgs;    // few rows: [seq] the first work group and the chunks of a block
+  float* scores;    // few rows with weights: [seq][kv head][row of the sequence][score_len], or null
   int score_len, score_rows;
 };
 
 __device__ __forceinline__ int64_t part_index(const PagedCall& a, int b, int t, int head, int split) {
   return ((static_cast<int64_t>(b) * a.bt.max_new + t) * a.n_heads + head) * a.n_splits + split;
+}
+
+__device__ __forceinline__ int64_t row_index(const PagedCall& a, int b, int t, int head) {
+  return (static_cast<int64_t>(b) * a.bt.max_new + t) * a.n_heads + head;
 }
 
 // The positions of a row block.
@@ -254,27 +261,30 @@ __device__ __forceinline__ float exact_row(const PagedCall& a, int b, int kh, in
   return o;
 }
 
-// exact_row for the rows of a block (those that `bad` marks, all without it), stored as
-// the block's own were.  Chunk `split` of the block's positions.
-template <typename TC, typename TI>
-__device__ __forceinline__ void exact_rows(int b, int kh, int rb, int split, int rows, const unsigned char* bad, float* s_q, float* s_p, float* s_red) {
+// exact_row for the rows of a block over positions [c0, c1) (the rows that `bad` marks,
+// all without it), stored as the block's own were: at part_at(i, t, head) unless final.
+template <typename TC, typename TI, class PartAt>
+__device__ __forceinline__ void exact_rows(int b, int kh, int rb, int rows, int c0, int c1, bool final, const unsigned char* bad, float* s_q, float* s_p,
+                                           float* s_red, const PartAt& part_at) {
   const PagedCall& a = call_again();
   const int tid = threadIdx.x, hd = a.kv.hd;
   const SeqRows sr = seq_rows(a.bt, b);
-  const RowBlock blk = row_block(a, b, rb, sr, seq_len(a.bt, a.kv, b));
-  const int c0 = blk.keys.lo + split * a.chunk, c1 = min(blk.keys.hi, c0 + a.chunk);
+  const int pos0 = seq_len(a.bt, a.kv, b) - sr.given, r_end = sr.n * a.group;
 #pragma unroll 1
-  for (int i = 0; i < rows && rb * rows + i < blk.r_end; ++i) {
+  for (int i = 0; i < rows && rb * rows + i < r_end; ++i) {
     if (bad && !bad[i]) continue;
     const int r = rb * rows + i, t = r / a.group, head = kh * a.group + r - t * a.group;
     float2 mz;
-    const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + t, head, blk.pos0 + t, c0, c1, s_q, s_p, s_red, &mz);
-    const int64_t at = part_index(a, b, t, head, split);
+    const float o = exact_row<TC, TI>(a, b, kh, sr.r0 + t, head, pos0 + t, c0, c1, s_q, s_p, s_red, &mz);
+    const int64_t at = part_at(a, i, t, head);
     if (tid < hd) {
-      if (a.n_splits == 1) static_cast<TI*>(a.out)[(sr.r0 + t) * a.out_stride + head * hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
+      if (final) static_cast<TI*>(a.out)[(sr.r0 + t) * a.out_stride + head * hd + tid] = static_cast<TI>(mz.y == 0.0f ? 0.0f : o / mz.y);
       else a.part_o[at * hd + tid] = o;
     }
-    if (tid == 0 && a.part_mz) a.part_mz[at] = mz;
+    if (tid == 0) {
+      if (a.part_mz) a.part_mz[at] = mz;
+      if (final && a.row_mz) a.row_mz[row_index(a, b, t, head)] = mz;
+    }
   }
 }
 
