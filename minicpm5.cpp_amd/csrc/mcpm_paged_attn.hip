@@ -30,7 +30,7 @@ constexpr int FEW_ROWS = 16;
 constexpr int FEW_STEP = 32;                // positions of a wave's step
 constexpr int FEW_ROUND = 4 * FEW_STEP;     // of a work group's
 constexpr int FEW_MAX_ROUNDS = 16;          // rounds of a work group, at most: its table of pages is in LDS
-constexpr int FEW_TARGET = 1, FEW_TARGET_64 = 4;  // work groups per CU that the work is shared among; heads of up to 64
+constexpr int FEW_TARGET = 1, FEW_TARGET_64 = 4;  // work groups per CU that the work is shared among
 constexpr int PROMPT_TARGET = 1;            // work groups per CU that a prompt's length is split for
 constexpr int PROMPT_MIN_CHUNK = 512;
 constexpr int FEW_MOST = 32;                // new tokens x group up to which these kernels run
@@ -55,8 +55,13 @@ struct FewTile16 {
     u32x4 w4;
     u32x2 w2;
   };
-  V8 k[2][KS];
-  VRow v[8][VH];
+  // A step's rows of K and V.  Two sets, where the registers allow: one is on its way
+  // while the other is used.
+  struct Rows {
+    V8 k[2][KS];
+    VRow v[8][VH];
+  };
+  static constexpr bool AHEAD = DP <= 128;
 
   // Rows of 32 bits over halves are brought to a top exponent of 8 by a power of
   // two, so that neither term leaves a half's range; products take it back.
@@ -95,29 +100,29 @@ struct FewTile16 {
 #pragma unroll
     for (int j = 0; j < NO; ++j) o[j] = f32x4{0, 0, 0, 0};
   }
-  __device__ __forceinline__ void load_k(int t, const TC* row, int hd) {
+  static __device__ __forceinline__ void load_k(Rows& x, int t, const TC* row, int hd) {
     const int g = (threadIdx.x >> 4) & 3;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k[t][s] = *reinterpret_cast<const V8*>(row + min(32 * s + 8 * g, hd - 8));
+    for (int s = 0; s < KS; ++s) x.k[t][s] = *reinterpret_cast<const V8*>(row + min(32 * s + 8 * g, hd - 8));
   }
-  __device__ __forceinline__ void load_v(int i, const TC* row, int hd) {
+  static __device__ __forceinline__ void load_v(Rows& x, int i, const TC* row, int hd) {
     const int m = threadIdx.x & 15;
 #pragma unroll
     for (int h = 0; h < VH; ++h) {
       const TC* p = row + min(16 * VW * h + VW * m, hd - VW);
-      if constexpr (VW == 8) v[i][h].w4 = *reinterpret_cast<const u32x4*>(p);
-      else v[i][h].w2 = *reinterpret_cast<const u32x2*>(p);
+      if constexpr (VW == 8) x.v[i][h].w4 = *reinterpret_cast<const u32x4*>(p);
+      else x.v[i][h].w2 = *reinterpret_cast<const u32x2*>(p);
     }
   }
-  __device__ __forceinline__ f32x4 scores(int t) {
+  __device__ __forceinline__ f32x4 scores(const Rows& x, int t) const {
     f32x4 s{0, 0, 0, 0};
 #pragma unroll
     for (int n = NT - 1; n >= 0; --n)
 #pragma unroll
-      for (int i = 0; i < KS; ++i) s = Half<TC>::mma16(k[t][i], q[n][i], s);
+      for (int i = 0; i < KS; ++i) s = Half<TC>::mma16(x.k[t][i], q[n][i], s);
     return s;
   }
-  __device__ __forceinline__ void add(const float (&p)[8]) {
+  __device__ __forceinline__ void add(const Rows& x, const float (&p)[8]) {
     V8 t[NT];
     split_terms<TC, NT>(p, t);
 #pragma unroll
@@ -127,8 +132,8 @@ struct FewTile16 {
         u32x4 lo, hi;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          lo[r] = __builtin_amdgcn_perm(v[2 * r + 1][h].w[w], v[2 * r][h].w[w], 0x05040100u);
-          hi[r] = __builtin_amdgcn_perm(v[2 * r + 1][h].w[w], v[2 * r][h].w[w], 0x07060302u);
+          lo[r] = __builtin_amdgcn_perm(x.v[2 * r + 1][h].w[w], x.v[2 * r][h].w[w], 0x05040100u);
+          hi[r] = __builtin_amdgcn_perm(x.v[2 * r + 1][h].w[w], x.v[2 * r][h].w[w], 0x07060302u);
         }
         const V8 a0 = __builtin_bit_cast(V8, lo), a1 = __builtin_bit_cast(V8, hi);
         const int j = h * VW + 2 * w;
@@ -156,8 +161,12 @@ struct FewTile<__bf16, TI, DP> : FewTile16<__bf16, TI, DP> {};
 template <int DP>
 struct FewTile<float, float, DP> {
   static constexpr int KS = DP / 16, VH = DP / 64, NO = DP / 16;
-  f32x4 q[KS], o[NO], k[2][KS], v[8][VH];
+  f32x4 q[KS], o[NO];
   float mul;
+  struct Rows {
+    f32x4 k[2][KS], v[8][VH];
+  };
+  static constexpr bool AHEAD = DP <= 128;
   __device__ __forceinline__ void load_q(const float* row, int hd, float score_mul) {
     const int g = (threadIdx.x >> 4) & 3;
     mul = score_mul;
@@ -168,31 +177,31 @@ struct FewTile<float, float, DP> {
       o[s] = f32x4{0, 0, 0, 0};
     }
   }
-  __device__ __forceinline__ void load_k(int t, const float* row, int hd) {
+  static __device__ __forceinline__ void load_k(Rows& x, int t, const float* row, int hd) {
     const int g = (threadIdx.x >> 4) & 3;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) k[t][s] = *reinterpret_cast<const f32x4*>(row + min(16 * s + 4 * g, hd - 4));
+    for (int s = 0; s < KS; ++s) x.k[t][s] = *reinterpret_cast<const f32x4*>(row + min(16 * s + 4 * g, hd - 4));
   }
-  __device__ __forceinline__ void load_v(int i, const float* row, int hd) {
+  static __device__ __forceinline__ void load_v(Rows& x, int i, const float* row, int hd) {
     const int m = threadIdx.x & 15;
 #pragma unroll
-    for (int h = 0; h < VH; ++h) v[i][h] = *reinterpret_cast<const f32x4*>(row + min(64 * h + 4 * m, hd - 4));
+    for (int h = 0; h < VH; ++h) x.v[i][h] = *reinterpret_cast<const f32x4*>(row + min(64 * h + 4 * m, hd - 4));
   }
-  __device__ __forceinline__ f32x4 scores(int t) {
+  __device__ __forceinline__ f32x4 scores(const Rows& x, int t) const {
     f32x4 s{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < KS; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k[t][i][c], q[i][c], s, 0, 0, 0);
+      for (int c = 0; c < 4; ++c) s = __builtin_amdgcn_mfma_f32_16x16x4f32(x.k[t][i][c], q[i][c], s, 0, 0, 0);
     return s;
   }
-  __device__ __forceinline__ void add(const float (&p)[8]) {
+  __device__ __forceinline__ void add(const Rows& x, const float (&p)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int h = 0; h < VH; ++h)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) o[4 * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][h][c], p[i], o[4 * h + c], 0, 0, 0);
+        for (int c = 0; c < 4; ++c) o[4 * h + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[i][h][c], p[i], o[4 * h + c], 0, 0, 0);
   }
   static __device__ __forceinline__ int d_of(int j, int i) {
     const int g = (threadIdx.x >> 4) & 3;
@@ -275,7 +284,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   __shared__ int s_bad;
   extern __shared__ int64_t s_off[];
   const PagedView& kv = a.kv;
-  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, n16 = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
   __shared__ Share s_share;
   __shared__ int64_t s_sum[2][4];
   Share sh;
@@ -322,15 +331,19 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   // Rows of one block differ in position by up to 15 tokens: a step that lies
   // before all of them and inside every window needs no masks.
   const bool plain = !a.rl.docs && !bad_pages && fb.first >= 0;
-  for (int p0 = c0 + wv * FEW_STEP; p0 < c1; p0 += FEW_ROUND) {
+  typedef FewTile<TC, TI, DP> Tile;
+  typedef typename Tile::Rows Rows;
+  auto load = [&](Rows& x, int p0) {
 #pragma unroll
-    for (int T = 0; T < 2; ++T) tile.load_k(T, kc + offset(p0 + 16 * T + n16), kv.hd);
+    for (int T = 0; T < 2; ++T) Tile::load_k(x, T, kc + offset(p0 + 16 * T + n16), kv.hd);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) tile.load_v(i, vc + offset(p0 + 16 * (i >> 2) + 4 * g + (i & 3)), kv.hd);
+    for (int i = 0; i < 8; ++i) Tile::load_v(x, i, vc + offset(p0 + 16 * (i >> 2) + 4 * g + (i & 3)), kv.hd);
+  };
+  auto use = [&](const Rows& rows, int p0) {
     float s[8];
 #pragma unroll
     for (int T = 0; T < 2; ++T) {
-      const f32x4 x = tile.scores(T);
+      const f32x4 x = tile.scores(rows, T);
 #pragma unroll
       for (int i = 0; i < 4; ++i) s[4 * T + i] = x[i];
     }
@@ -372,7 +385,27 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
       p[i] = __builtin_amdgcn_exp2f(s[i] - m);
       z += p[i];
     }
-    tile.add(p);
+    tile.add(rows, p);
+  };
+  const int begin = c0 + wv * FEW_STEP;
+  if constexpr (Tile::AHEAD) {
+    Rows x, y;
+    if (begin < c1) load(x, begin);
+    for (int p0 = begin; p0 < c1; p0 += 2 * FEW_ROUND) {
+      if (p0 + FEW_ROUND < c1) load(y, p0 + FEW_ROUND);
+      __builtin_amdgcn_sched_barrier(0);
+      use(x, p0);
+      if (p0 + FEW_ROUND >= c1) break;
+      if (p0 + 2 * FEW_ROUND < c1) load(x, p0 + 2 * FEW_ROUND);
+      __builtin_amdgcn_sched_barrier(0);
+      use(y, p0 + FEW_ROUND);
+    }
+  } else {
+    Rows x;
+    for (int p0 = begin; p0 < c1; p0 += FEW_ROUND) {
+      load(x, p0);
+      use(x, p0);
+    }
   }
 
   // the waves' partials, joined in LDS
@@ -622,7 +655,11 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
   size_t parts;
   if (p.few) {
     const int64_t rounds = (span + FEW_ROUND - 1) / FEW_ROUND;
-    const int per_cu = kv.hd <= 64 ? FEW_TARGET_64 : FEW_TARGET;
+    // One work group per CU keeps its memory busy, and more of them start later (two
+    // caches of 100,003, heads of 128: 50 us, 61 with two).  Heads of up to 64 leave room
+    // for more at once, which evens out many ragged sequences of costly rules (48 with
+    // weights and a cap: 90 us instead of 97; a single one of 40,000 loses, 33 for 25).
+    const int per_cu = kv.hd <= 64 && blocks >= n_cu ? FEW_TARGET_64 : FEW_TARGET;
     p.chunk = per_cu * n_cu;
     // few_share gives a sequence a work group more than its share, at most, and none more than FEW_MAX_ROUNDS
     const int64_t most = std::max<int64_t>(p.chunk, blocks * ((rounds + FEW_MAX_ROUNDS - 1) / FEW_MAX_ROUNDS)) + blocks;
