@@ -29,7 +29,7 @@ namespace {
 constexpr int FEW_ROWS = 16;
 constexpr int FEW_STEP = 32;                // positions of a wave's step
 constexpr int FEW_ROUND = 4 * FEW_STEP;     // of a work group's
-constexpr int FEW_MAX_ROUNDS = 16;          // rounds of a work group, at most: its table of pages is in LDS
+constexpr int FEW_PAGES = 2048;             // a work group's table of pages in LDS, at most
 constexpr int FEW_TARGET = 1, FEW_TARGET_64 = 4;  // work groups per CU that the work is shared among
 constexpr int PROMPT_TARGET = 1;            // work groups per CU that a prompt's length is split for
 constexpr int PROMPT_MIN_CHUNK = 512;
@@ -222,6 +222,9 @@ __device__ __forceinline__ SeqWork seq_work(const PagedCall& a, int b) {
   return SeqWork{k, k.hi > k.lo ? (k.hi - k.lo + FEW_ROUND - 1) / FEW_ROUND : 1, (sr.n * a.group + FEW_ROWS - 1) / FEW_ROWS};
 }
 
+// Rounds of a work group, at most.
+__host__ __device__ inline int few_max_rounds(const PagedView& kv) { return FEW_PAGES / FEW_ROUND << kv.page_shift; }
+
 // Which part of which sequence this work group has.  The host knows a bound of the
 // lengths only, and they are ragged: every work group sums up the rounds of all
 // sequences and takes its share of them, the same number of rounds (the last of a
@@ -242,7 +245,7 @@ __device__ __forceinline__ bool few_share(const PagedCall& a, Share* s_share, in
   if (tid == 0) s_share->b = -1;
   __syncthreads();
   const int64_t total = s_wave[0][0] + s_wave[0][1] + s_wave[0][2] + s_wave[0][3];
-  const int rounds = static_cast<int>(min(max((total + a.chunk - 1) / a.chunk, static_cast<int64_t>(1)), static_cast<int64_t>(FEW_MAX_ROUNDS)));
+  const int rounds = static_cast<int>(min(max((total + a.chunk - 1) / a.chunk, static_cast<int64_t>(1)), static_cast<int64_t>(few_max_rounds(a.kv))));
   int64_t base = 0;
   for (int b0 = 0; b0 < n; b0 += 256) {
     const int b = b0 + tid;
@@ -546,40 +549,47 @@ __global__ void __launch_bounds__(256) k_attention_join(const PagedCall a) {
 }
 
 // The weights of 1024 positions of a kv head from the scores: a lane has four, and sums
-// the rows in order.  The rows' (m, z) are joined from the partials here too, so that
-// this runs beside the join.
-__device__ __forceinline__ void add_weights(const PagedCall& a, int kh, int chunk, int b, char* lds) {
+// the rows in order.  The rows' (m, z) are joined from the partials here too (16 lanes a
+// row), so that this runs beside the join.
+__device__ __forceinline__ void add_weights(const PagedCall& a, const KeyRange& keys, int kh, int chunk, int b, char* lds) {
   float2* s_mz = reinterpret_cast<float2*>(lds);
   const int tid = threadIdx.x, j = chunk * 1024 + tid * 4;
-  const int len = seq_len(a.bt, a.kv, b);
-  if (chunk * 1024 >= len) return;
   const SeqRows sr = seq_rows(a.bt, b);
-  const SeqWork w = seq_work(a, b);
-  const int rows = sr.n * a.group;
+  const int rows = sr.n * a.group, lane_row = tid / FEW_ROWS, part = tid % FEW_ROWS;
   const float* sc = a.scores + (static_cast<int64_t>(b) * a.kv.n_kv_heads + kh) * a.score_rows * a.score_len + j;
   f32x4 sum{0, 0, 0, 0};
   for (int r0 = 0; r0 < rows; r0 += FEW_ROWS) {
-    __syncthreads();
-    if (tid < FEW_ROWS && r0 + tid < rows) {
-      const int t = (r0 + tid) / a.group;
-      const Parts p = parts_of<true>(a, b, sr, t, kh * a.group + r0 + tid - t * a.group);
-      float2 mz = make_float2(MAX_START, 0.0f);
-      for (int k = 0; k < p.n; ++k) join_mz(mz, a.part_mz[p.at + k * p.stride]);
-      s_mz[tid] = make_float2(mz.x, mz.y == 0.0f ? 0.0f : 1.0f / mz.y);
-    }
-    __syncthreads();
-    if (j < w.keys.hi)
-      for (int i = 0; i < FEW_ROWS && r0 + i < rows; ++i) {
-        const f32x4 s = *reinterpret_cast<const f32x4*>(sc + static_cast<int64_t>(r0 + i) * a.score_len);
-        const float2 mz = s_mz[i];
+    constexpr int AT_ONCE = 4;  // rows whose scores are asked for together
+    f32x4 s[AT_ONCE];
+    auto ask = [&](int i0) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (j + k >= w.keys.lo && j + k < w.keys.hi) sum[k] += __builtin_amdgcn_exp2f(s[k] - mz.x) * mz.y;
+      for (int i = 0; i < AT_ONCE; ++i)
+        s[i] = j < keys.hi && r0 + i0 + i < rows ? *reinterpret_cast<const f32x4*>(sc + static_cast<int64_t>(r0 + i0 + i) * a.score_len) : f32x4{0, 0, 0, 0};
+    };
+    ask(0);
+    float2 mz = make_float2(MAX_START, 0.0f);
+    if (r0 + lane_row < rows) {
+      const int t = (r0 + lane_row) / a.group;
+      const Parts p = parts_of<true>(a, b, sr, t, kh * a.group + r0 + lane_row - t * a.group);
+      for (int k = part; k < p.n; k += FEW_ROWS) join_mz(mz, a.part_mz[p.at + k * p.stride]);
+    }
+    for (int x = 1; x < FEW_ROWS; x <<= 1) join_mz(mz, make_float2(__shfl_xor(mz.x, x), __shfl_xor(mz.y, x)));
+    __syncthreads();
+    if (part == 0) s_mz[lane_row] = make_float2(mz.x, mz.y == 0.0f ? 0.0f : 1.0f / mz.y);
+    __syncthreads();
+    for (int i0 = 0; i0 < FEW_ROWS && r0 + i0 < rows; i0 += AT_ONCE) {
+      if (i0) ask(i0);
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const float2 f = s_mz[i0 + i];  // past the last row: 1 / z is 0
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sum[k] += j + k >= keys.lo && j + k < keys.hi ? __builtin_amdgcn_exp2f(s[i][k] - f.x) * f.y : 0.0f;
       }
+    }
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    if (j + k >= w.keys.hi) break;
+    if (j + k < keys.lo || j + k >= keys.hi) continue;
     const int page = page_of(a.bt, a.kv, b, j + k);
     if (page >= 0) *weight_of(a.kv, page, j + k, kh) += sum[k];
   }
@@ -588,50 +598,101 @@ __device__ __forceinline__ void add_weights(const PagedCall& a, int kh, int chun
 // After the few-row kernel, in one launch: `join_blocks` work groups a sequence join its
 // rows, the others add up the weights.
 template <typename TI, int DP, int ROWS>
-__global__ void __launch_bounds__(256) k_few_finish(const PagedCall a, int join_blocks) {
+__global__ void __launch_bounds__(256) k_few_finish(const PagedCall a, int join_blocks, int weight_blocks) {
   __shared__ __attribute__((aligned(16))) char lds[JOIN_LDS];
-  const int x = blockIdx.x, b = blockIdx.y;
-  if (x < join_blocks) join_rows<true, TI, DP, ROWS>(a, x, b, lds);
-  else add_weights(a, (x - join_blocks) % a.kv.n_kv_heads, (x - join_blocks) / a.kv.n_kv_heads, b, lds);
+  const int x = blockIdx.x, b = blockIdx.y, w = x - join_blocks;
+  if (w < 0) return join_rows<true, TI, DP, ROWS>(a, x, b, lds);
+  const KeyRange keys = seq_work(a, b).keys;
+  for (int c = keys.lo / 1024 + w / a.kv.n_kv_heads; c * 1024 < keys.hi; c += weight_blocks) add_weights(a, keys, w % a.kv.n_kv_heads, c, b, lds);
 }
 
-__device__ __forceinline__ float simple_score(const RuleView& rl, float slope, float dot, int pos, int j) {
-  const ScoreRule r = score_rule(rl);
-  return score_of(r, dot, r.mul) - slope * LOG2E * fabsf(static_cast<float>(pos - j));
-}
-
-// The same for prompts, whose scores are formed once more: a lane per position.
-template <typename TC, typename TI>
-__global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
+// The same where the scores were not kept: they are formed once more.  A work group has
+// 64 positions of a kv head, whose keys stay in registers while the rows that may see them
+// go by, 16 at a time, the four waves in turn.
+constexpr int WEIGHT_KEYS = 64;
+template <typename TC, typename TI, int DP>
+__device__ __forceinline__ void weights_again(const PagedCall& a, int p0, int kh, int b) {
+  typedef FewTile<TC, TI, DP> Tile;
+  constexpr int NK = WEIGHT_KEYS / 32;
+  __shared__ float s_sum[4][WEIGHT_KEYS];
   const PagedView& kv = a.kv;
-  const int j = blockIdx.x * 256 + threadIdx.x, kh = blockIdx.y, b = blockIdx.z, hd = kv.hd;
+  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6), n16 = lane & 15, g = lane >> 4;
   const int len = seq_len(a.bt, kv, b);
   const SeqRows sr = seq_rows(a.bt, b);
-  if (j >= len) return;
-  const int page = page_of(a.bt, kv, b, j);
-  if (page < 0) return;
-  const TC* k = reinterpret_cast<const TC*>(kv.k) + elem_of(kv, page, j, kh);
-  float sum = 0.0f;
-  for (int t = 0; t < sr.n; ++t) {
-    const int pos = len - sr.given + t;
-    const RowRule rr = row_rule(a.rl, b, pos, len);
-    if (!in_span(rr, j) || tag_of(a.rl, a.bt, kv, b, j, false) != rr.tag) continue;
-    for (int h = kh * a.group; h < kh * a.group + a.group; ++h) {
-      const TI* q = static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + h * hd;
-      float d = 0.0f;
-      for (int i = 0; i < hd; ++i) d = __builtin_fmaf(static_cast<float>(q[i]), static_cast<float>(k[i]), d);
-      const float2 r = a.row_mz[row_index(a, b, t, h)];
-      if (r.y != 0.0f) sum += __builtin_amdgcn_exp2f(simple_score(a.rl, a.rl.slopes ? a.rl.slopes[h] : 0.0f, d, pos, j) - r.x) / r.y;
+  // tokens [t0, t1) may see some of the positions
+  const int pos0 = len - sr.given, last = p0 + WEIGHT_KEYS - 1;
+  const int t0 = a.rl.prefix && a.rl.prefix[b] > p0 ? 0 : max(p0 - pos0, 0);
+  const int t1 = a.rl.window > 0 ? static_cast<int>(min(static_cast<int64_t>(sr.n), max(static_cast<int64_t>(last) - pos0 + a.rl.window, static_cast<int64_t>(0)))) : sr.n;
+  if (t0 >= t1) return;
+
+  typename Tile::Rows keys[NK];
+  int tag[NK][8];
+#pragma unroll
+  for (int n = 0; n < NK; ++n) {
+#pragma unroll
+    for (int T = 0; T < 2; ++T) {
+      const int j = min(p0 + 32 * n + 16 * T + n16, len - 1);
+      Tile::load_k(keys[n], T, reinterpret_cast<const TC*>(kv.k) + elem_of(kv, max(page_of(a.bt, kv, b, j), 0), j, kh), kv.hd);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) tag[n][i] = tag_of(a.rl, a.bt, kv, b, min(p0 + 32 * n + 16 * (i >> 2) + 4 * g + (i & 3), len - 1), true);
+  }
+  const ScoreRule rule = score_rule(a.rl);
+  float sum[NK][8] = {};
+  for (int r0 = t0 * a.group + 16 * wv; r0 < t1 * a.group; r0 += 64) {
+    const int r = r0 + n16;
+    const bool in = r < t1 * a.group;
+    const int t = in ? r / a.group : t0, head = kh * a.group + (in ? r - t * a.group : 0), pos = pos0 + t;
+    const float2 mz = a.row_mz[row_index(a, b, t, head)];
+    const float inv = in && mz.y != 0.0f ? 1.0f / mz.y : 0.0f;
+    const RowRule rr = row_rule(a.rl, b, in ? pos : -1, len);
+    const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
+    Tile tile;
+    tile.load_q(static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + head * kv.hd, kv.hd, rule.mul);
+#pragma unroll
+    for (int n = 0; n < NK; ++n) {
+      float s[8];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        const f32x4 x = tile.scores(keys[n], T);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * T + i] = x[i];
+      }
+      scores_of<8>(rule, s, tile.mul);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = p0 + 32 * n + 16 * (i >> 2) + 4 * g + (i & 3);
+        const float x = s[i] - slope * fabsf(static_cast<float>(pos - j));
+        sum[n][i] += in_span(rr, j) && tag[n][i] == rr.tag ? __builtin_amdgcn_exp2f(x - mz.x) * inv : 0.0f;
+      }
     }
   }
-  *weight_of(kv, page, j, kh) += sum;
+#pragma unroll
+  for (int n = 0; n < NK; ++n)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float x = sum[n][i];
+      for (int k = 1; k < 16; k <<= 1) x += __shfl_xor(x, k);
+      if (n16 == 0) s_sum[wv][32 * n + 16 * (i >> 2) + 4 * g + (i & 3)] = x;
+    }
+  __syncthreads();
+  if (tid < WEIGHT_KEYS && p0 + tid < len) {
+    const int page = page_of(a.bt, kv, b, p0 + tid);
+    if (page >= 0) *weight_of(kv, page, p0 + tid, kh) += s_sum[0][tid] + s_sum[1][tid] + s_sum[2][tid] + s_sum[3][tid];
+  }
+  __syncthreads();
+}
+template <typename TC, typename TI, int DP>
+__global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
+  const int len = seq_len(a.bt, a.kv, blockIdx.z);
+  for (int p0 = blockIdx.x * WEIGHT_KEYS; p0 < len; p0 += gridDim.x * WEIGHT_KEYS) weights_again<TC, TI, DP>(a, p0, blockIdx.y, blockIdx.z);
 }
 
 // How a call is cut into work groups.  Up to FEW_MOST rows of a sequence and kv
 // head take the 16-row kernel, more the prompt kernel.
 struct Plan {
   bool few;
-  int block_rows, n_blocks, chunk, n_splits, grid, score_len;
+  int block_rows, n_blocks, chunk, n_splits, grid, lds_pages, score_len;
   size_t o_bytes, mz_bytes, row_bytes, seq_bytes, score_bytes;
   size_t bytes() const { return o_bytes + mz_bytes + row_bytes + seq_bytes + score_bytes; }
 };
@@ -661,8 +722,10 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
     // weights and a cap: 90 us instead of 97; a single one of 40,000 loses, 33 for 25).
     const int per_cu = kv.hd <= 64 && blocks >= n_cu ? FEW_TARGET_64 : FEW_TARGET;
     p.chunk = per_cu * n_cu;
-    // few_share gives a sequence a work group more than its share, at most, and none more than FEW_MAX_ROUNDS
-    const int64_t most = std::max<int64_t>(p.chunk, blocks * ((rounds + FEW_MAX_ROUNDS - 1) / FEW_MAX_ROUNDS)) + blocks;
+    // few_share gives a block a work group more than its share, at most, and none more than max_rounds
+    const int max_rounds = few_max_rounds(kv);
+    const int64_t most = std::max<int64_t>(p.chunk, blocks * ((rounds + max_rounds - 1) / max_rounds)) + blocks;
+    p.lds_pages = static_cast<int>(std::min<int64_t>(FEW_PAGES, span >> kv.page_shift) + 2);
     const int64_t grid = std::min(most, blocks * rounds);
     p.grid = grid > INT_MAX ? -1 : static_cast<int>(grid);
     p.n_splits = rounds > 1 ? 2 : 1;
@@ -686,21 +749,27 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
 }
 
 template <typename TC, typename TI, int DP>
-hipError_t few(const PagedCall& a, int grid, hipStream_t s) {
-  const size_t lds = (static_cast<size_t>(FEW_MAX_ROUNDS * FEW_ROUND >> a.kv.page_shift) + 2) * sizeof(int64_t);
-  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(grid), dim3(256), lds, s, a);
+hipError_t few(const PagedCall& a, const Plan& p, hipStream_t s) {
+  hipLaunchKernelGGL((k_attention_few<TC, TI, DP>), dim3(p.grid), dim3(256), p.lds_pages * sizeof(int64_t), s, a);
   return hipGetLastError();
 }
 template <typename TC, typename TI>
-hipError_t few(const PagedCall& a, int grid, hipStream_t s) {
-  return a.kv.hd <= 64 ? few<TC, TI, 64>(a, grid, s) : a.kv.hd <= 128 ? few<TC, TI, 128>(a, grid, s) : few<TC, TI, 256>(a, grid, s);
+hipError_t few(const PagedCall& a, const Plan& p, hipStream_t s) {
+  return a.kv.hd <= 64 ? few<TC, TI, 64>(a, p, s) : a.kv.hd <= 128 ? few<TC, TI, 128>(a, p, s) : few<TC, TI, 256>(a, p, s);
 }
-hipError_t launch_attention_few(const PagedCall& a, int grid, int kv_type, int io_type, hipStream_t s) {
-  if (grid < 0) return hipErrorInvalidValue;
+hipError_t launch_attention_few(const PagedCall& a, const Plan& p, int kv_type, int io_type, hipStream_t s) {
+  if (p.grid < 0) return hipErrorInvalidValue;
   const bool f32 = io_type == MCPM_TYPE_F32;
-  if (kv_type == MCPM_TYPE_F32) return few<float, float>(a, grid, s);
-  if (kv_type == MCPM_TYPE_F16) return f32 ? few<_Float16, float>(a, grid, s) : few<_Float16, _Float16>(a, grid, s);
-  return f32 ? few<__bf16, float>(a, grid, s) : few<__bf16, __bf16>(a, grid, s);
+  if (kv_type == MCPM_TYPE_F32) return few<float, float>(a, p, s);
+  if (kv_type == MCPM_TYPE_F16) return f32 ? few<_Float16, float>(a, p, s) : few<_Float16, _Float16>(a, p, s);
+  return f32 ? few<__bf16, float>(a, p, s) : few<__bf16, __bf16>(a, p, s);
+}
+
+// Work groups for each (sequence, kv head) of a weights' sum over `most` slices: per_cu
+// of them per CU in all, so that a bound far above the lengths costs no idle ones.
+int slices_of(int most, int per_cu, const PagedCall& a, int n_cu) {
+  const int64_t pairs = static_cast<int64_t>(a.bt.n_seq) * a.kv.n_kv_heads;
+  return static_cast<int>(std::min<int64_t>(most, (static_cast<int64_t>(per_cu) * n_cu + pairs - 1) / pairs));
 }
 
 // What follows the main kernel: the join where rows are in parts, the weights' sum
@@ -716,9 +785,10 @@ hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
     if (side) hipLaunchKernelGGL((k_attention_join<TI, DP, MOST>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_attention_join<TI, DP, 1>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
   } else {
-    const dim3 grid(joins + (a.scores ? (a.score_len + 1023) / 1024 * a.kv.n_kv_heads : 0), a.bt.n_seq);
-    if (side) hipLaunchKernelGGL((k_few_finish<TI, DP, MOST>), grid, dim3(256), 0, s, a, joins);
-    else hipLaunchKernelGGL((k_few_finish<TI, DP, 1>), grid, dim3(256), 0, s, a, joins);
+    const int weights = a.scores ? slices_of((a.score_len + 1023) / 1024, 8, a, n_cu) : 0;
+    const dim3 grid(joins + weights * a.kv.n_kv_heads, a.bt.n_seq);
+    if (side) hipLaunchKernelGGL((k_few_finish<TI, DP, MOST>), grid, dim3(256), 0, s, a, joins, weights);
+    else hipLaunchKernelGGL((k_few_finish<TI, DP, 1>), grid, dim3(256), 0, s, a, joins, weights);
   }
   return hipGetLastError();
 }
@@ -727,10 +797,15 @@ hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
   return a.kv.hd <= 64 ? finish<TI, 64>(a, few, n_cu, s) : a.kv.hd <= 128 ? finish<TI, 128>(a, few, n_cu, s) : finish<TI, 256>(a, few, n_cu, s);
 }
 
-template <typename TC, typename TI>
-hipError_t prompt_weight(const PagedCall& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_prompt_weight<TC, TI>), dim3((a.score_len + 255) / 256, a.kv.n_kv_heads, a.bt.n_seq), dim3(256), 0, s, a);
+template <typename TC, typename TI, int DP>
+hipError_t prompt_weight(const PagedCall& a, int n_cu, hipStream_t s) {
+  const dim3 grid(slices_of((a.score_len + WEIGHT_KEYS - 1) / WEIGHT_KEYS, 32, a, n_cu), a.kv.n_kv_heads, a.bt.n_seq);
+  hipLaunchKernelGGL((k_prompt_weight<TC, TI, DP>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
+}
+template <typename TC, typename TI>
+hipError_t prompt_weight(const PagedCall& a, int n_cu, hipStream_t s) {
+  return a.kv.hd <= 64 ? prompt_weight<TC, TI, 64>(a, n_cu, s) : a.kv.hd <= 128 ? prompt_weight<TC, TI, 128>(a, n_cu, s) : prompt_weight<TC, TI, 256>(a, n_cu, s);
 }
 
 }  // namespace
@@ -758,7 +833,7 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
   a.scores = reinterpret_cast<float*>(take(p.score_bytes));
   a.score_len = p.score_len;
   a.score_rows = bt.max_new * group;
-  hipError_t e = p.few ? launch_attention_few(a, p.grid, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
+  hipError_t e = p.few ? launch_attention_few(a, p, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
   if (e != hipSuccess) return e;
   if (p.n_splits > 1 || a.scores) {
     e = io_type == MCPM_TYPE_F32 ? finish<float>(a, p.few, n_cu, s) : io_type == MCPM_TYPE_F16 ? finish<_Float16>(a, p.few, n_cu, s) : finish<__bf16>(a, p.few, n_cu, s);
@@ -766,9 +841,9 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
   }
   if (!kv.weight || a.scores || !p.score_len) return hipSuccess;
   const bool f32 = io_type == MCPM_TYPE_F32;
-  if (kv_type == MCPM_TYPE_F32) return prompt_weight<float, float>(a, s);
-  if (kv_type == MCPM_TYPE_F16) return f32 ? prompt_weight<_Float16, float>(a, s) : prompt_weight<_Float16, _Float16>(a, s);
-  return f32 ? prompt_weight<__bf16, float>(a, s) : prompt_weight<__bf16, __bf16>(a, s);
+  if (kv_type == MCPM_TYPE_F32) return prompt_weight<float, float>(a, n_cu, s);
+  if (kv_type == MCPM_TYPE_F16) return f32 ? prompt_weight<_Float16, float>(a, n_cu, s) : prompt_weight<_Float16, _Float16>(a, n_cu, s);
+  return f32 ? prompt_weight<__bf16, float>(a, n_cu, s) : prompt_weight<__bf16, __bf16>(a, n_cu, s);
 }
 
 }  // namespace mcpm

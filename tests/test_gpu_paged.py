@@ -218,6 +218,43 @@ def test_prompt_long_past(ctx, t, io):
 
 
 @pytest.mark.parametrize("t,io", TYPES, ids=IDS)
+@pytest.mark.parametrize("heads", sorted(HEADS))
+def test_prompt_weights(ctx, heads, t, io):
+    """The weights that the rows of prompts add, also of chunks after a past."""
+    check_attention(ctx, heads, HEADS[heads], t, io, [70, 131, 9], [70, 40, 9], weight=True, seed=18)
+
+
+@pytest.mark.parametrize("rule", sorted(RULES))
+def test_weights_of_a_few_tokens_of_many_heads(ctx, rule):
+    """A few tokens of a large group after a long past: many rows, few of them tokens."""
+    lens, news = [1500, 300, 70], [5, 3, 5]
+    rules = make_rules(rule, 32, lens, np.random.default_rng(19))
+    check_attention(ctx, rule, (32, 2, 64), F16, F32, lens, news, page=64, rules=rules, weight=True, seed=19)
+
+
+def test_bounds_far_above_the_lengths(ctx):
+    """max_len and tables for caches far longer than these are: too many scores to keep, so that the weights are formed
+    from scores made again, and work groups for lengths that do not come."""
+    KH, hd, page, n_seq, per = 1, 8, 65536, 16, 12
+    rng = np.random.default_rng(20)
+    cache = R.Cache(F16, n_seq, page, KH, hd, rng=rng, weight=True)
+    cache.weight[:] = 0.0
+    tables = np.full((n_seq, per), -1, np.int32)
+    tables[:, 0] = rng.permutation(n_seq)
+    lens = [int(n) for n in rng.integers(3, 700, n_seq)]
+    for H, new in ((32, 1), (8, 3)):
+        q = R.store(rng.standard_normal((n_seq * new, H * hd)), F32)
+        news = [new] * n_seq
+        for max_len in (per * page, 1 << 30):
+            announce(f"bound {max_len} for lengths below 700, {new} new")
+            dev = Dev(ctx, cache, tables, lens, news, max_len=max_len)
+            got = run_attention(ctx, dev, q, F32, H, {})
+            want, bound, w, wb = R.attention(cache, tables, lens, news, q, F32, H, {})
+            assert (np.abs(got - want) <= bound).all()
+            assert (np.abs(dev.image("weight") - w) <= wb + 2.0 ** -23 * w).all()
+
+
+@pytest.mark.parametrize("t,io", TYPES, ids=IDS)
 def test_prompt_documents_of_many_tiles(ctx, t, io):
     """Documents longer than a tile of keys, so that tiles hold one alone; rows of no document between rows of one,
     in the same block of rows."""
