@@ -79,7 +79,7 @@ hipError_t launch_paged_append(const PagedView& kv, int kv_type, const BatchView
                                float rope_base, int n_cu, hipStream_t s);
 
 // Bytes of scratch that launch_paged_attention needs.
-size_t paged_attention_scratch(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu);
+size_t paged_attention_scratch(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type, int n_heads, int n_cu);
 hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type,
                                   void* out, int64_t out_stride, const void* q, int64_t q_stride, int n_heads,
                                   void* scratch, int n_cu, hipStream_t s);

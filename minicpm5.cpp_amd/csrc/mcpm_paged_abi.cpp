@@ -149,7 +149,7 @@ int mcpm_paged_attention(mcpm_ctx* c, void* out, int64_t out_stride, const void*
   if (!bt.n_seq || !bt.n_rows || !bt.max_new) return MCPM_OK;
   DeviceScope dev(c->device);
   MCPM_HIP(dev.status());
-  rc = ensure_paged_scratch(c, paged_attention_scratch(kvv, bt, rl, n_heads, c->n_cu));
+  rc = ensure_paged_scratch(c, paged_attention_scratch(kvv, kv->type, bt, rl, io_type, n_heads, c->n_cu));
   if (rc) return rc;
   MCPM_HIP(launch_paged_attention(kvv, kv->type, bt, rl, io_type, out, out_stride, q, q_stride, n_heads, c->d_paged, c->n_cu, c->stream));
   return MCPM_OK;

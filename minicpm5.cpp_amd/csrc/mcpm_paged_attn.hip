@@ -31,8 +31,6 @@ constexpr int FEW_STEP = 32;                // positions of a wave's step
 constexpr int FEW_ROUND = 4 * FEW_STEP;     // of a work group's
 constexpr int FEW_PAGES = 2048;             // a work group's table of pages in LDS, at most
 constexpr int FEW_TARGET = 1, FEW_TARGET_64 = 4;  // work groups per CU that the work is shared among
-constexpr int PROMPT_TARGET = 1;            // work groups per CU that a prompt's length is split for
-constexpr int PROMPT_MIN_CHUNK = 512;
 constexpr int FEW_MOST = 32;                // new tokens x group up to which these kernels run
 
 template <typename TC, typename TI, int DP>
@@ -699,7 +697,26 @@ struct Plan {
 size_t round16(size_t n) { return (n + 15) / 16 * 16; }
 constexpr size_t MOST_SCORES = size_t{1} << 30;  // bytes of kept scores, past which they are formed again
 
-Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu) {
+// Work groups per CU that a prompt's length is split for, and the shortest chunk.  A
+// split pays for its join where a tile of keys is dear: on the 32-bit matrix
+// instructions, 1/8 of the rate, anywhere (heads of 256, 200 tokens: 82 us whole, 48 in
+// chunks of 64), there with four work groups per CU, which even out the causal triangle
+// (heads of 128, 2400 tokens: 381 us with one, 240 with four; under a window, which has
+// no triangle, one: 164 us, 242 with four); with heads of 256 or 32-bit rows over a
+// 16-bit cache's heads of 128 in chunks of 128 (1000 tokens, 8 heads of 256: 124 us
+// whole, 82 split); not elsewhere (300 tokens, heads of 64: 12 us whole, 15 split), nor
+// where documents leave most of a chunk unseen (260 tokens in documents of 30, heads of
+// 256: 38 us whole, 44 split).
+struct PromptSplit {
+  int per_cu, least;
+};
+PromptSplit prompt_split(int kv_type, int io_type, int hd, const RuleView& rl) {
+  if (rl.docs) return {1, 512};
+  if (kv_type == MCPM_TYPE_F32) return {rl.window > 0 && !rl.prefix ? 1 : 4, 64};
+  return {1, hd > 128 || (hd > 64 && io_type == MCPM_TYPE_F32) ? 128 : 512};
+}
+
+Plan plan_of(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type, int n_heads, int n_cu) {
   Plan p{};
   const int group = n_heads / kv.n_kv_heads;
   const int64_t rows = static_cast<int64_t>(bt.max_new) * group;
@@ -732,8 +749,9 @@ Plan plan_of(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n
     parts = static_cast<size_t>(grid) * FEW_ROWS;
     p.seq_bytes = p.n_splits > 1 || kv.weight ? round16(bt.n_seq * sizeof(int2)) : 0;
   } else {
-    const int64_t want = std::max<int64_t>(1, PROMPT_TARGET * n_cu / blocks);
-    p.chunk = static_cast<int>((std::max<int64_t>((span + want - 1) / want, PROMPT_MIN_CHUNK) + 63) / 64 * 64);
+    const PromptSplit split = prompt_split(kv_type, io_type, kv.hd, rl);
+    const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(split.per_cu) * n_cu / blocks);
+    p.chunk = static_cast<int>((std::max<int64_t>((span + want - 1) / want, split.least) + 63) / 64 * 64);
     p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
     parts = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.n_splits;
   }
@@ -810,14 +828,14 @@ hipError_t prompt_weight(const PagedCall& a, int n_cu, hipStream_t s) {
 
 }  // namespace
 
-size_t paged_attention_scratch(const PagedView& kv, const BatchView& bt, const RuleView& rl, int n_heads, int n_cu) {
-  return plan_of(kv, bt, rl, n_heads, n_cu).bytes();
+size_t paged_attention_scratch(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type, int n_heads, int n_cu) {
+  return plan_of(kv, kv_type, bt, rl, io_type, n_heads, n_cu).bytes();
 }
 
 hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchView& bt, const RuleView& rl, int io_type,
                                   void* out, int64_t out_stride, const void* q, int64_t q_stride, int n_heads,
                                   void* scratch, int n_cu, hipStream_t s) {
-  const Plan p = plan_of(kv, bt, rl, n_heads, n_cu);
+  const Plan p = plan_of(kv, kv_type, bt, rl, io_type, n_heads, n_cu);
   const int group = n_heads / kv.n_kv_heads;
   char* sc = static_cast<char*>(scratch);
   auto take = [&](size_t bytes) {
