@@ -555,6 +555,14 @@ __device__ __forceinline__ void add_weights(const PagedCall& a, const KeyRange& 
   const SeqRows sr = seq_rows(a.bt, b);
   const int rows = sr.n * a.group, lane_row = tid / FEW_ROWS, part = tid % FEW_ROWS;
   const float* sc = a.scores + (static_cast<int64_t>(b) * a.kv.n_kv_heads + kh) * a.score_rows * a.score_len + j;
+  float* at[4];  // what the sum goes to, asked for ahead of it
+  float old[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int page = j + k >= keys.lo && j + k < keys.hi ? page_of(a.bt, a.kv, b, j + k) : -1;
+    at[k] = page >= 0 ? weight_of(a.kv, page, j + k, kh) : nullptr;
+    old[k] = at[k] ? *at[k] : 0.0f;
+  }
   f32x4 sum{0, 0, 0, 0};
   for (int r0 = 0; r0 < rows; r0 += FEW_ROWS) {
     constexpr int AT_ONCE = 4;  // rows whose scores are asked for together
@@ -586,11 +594,8 @@ __device__ __forceinline__ void add_weights(const PagedCall& a, const KeyRange& 
     }
   }
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    if (j + k < keys.lo || j + k >= keys.hi) continue;
-    const int page = page_of(a.bt, a.kv, b, j + k);
-    if (page >= 0) *weight_of(a.kv, page, j + k, kh) += sum[k];
-  }
+  for (int k = 0; k < 4; ++k)
+    if (at[k]) *at[k] = old[k] + sum[k];
 }
 
 // After the few-row kernel, in one launch: `join_blocks` work groups a sequence join its
@@ -690,7 +695,7 @@ __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
 // head take the 16-row kernel, more the prompt kernel.
 struct Plan {
   bool few;
-  int block_rows, n_blocks, chunk, n_splits, grid, lds_pages, score_len;
+  int block_rows, n_blocks, chunk, n_splits, grid, lds_pages, row_parts, score_len;
   size_t o_bytes, mz_bytes, row_bytes, seq_bytes, score_bytes;
   size_t bytes() const { return o_bytes + mz_bytes + row_bytes + seq_bytes + score_bytes; }
 };
@@ -746,13 +751,14 @@ Plan plan_of(const PagedView& kv, int kv_type, const BatchView& bt, const RuleVi
     const int64_t grid = std::min(most, blocks * rounds);
     p.grid = grid > INT_MAX ? -1 : static_cast<int>(grid);
     p.n_splits = rounds > 1 ? 2 : 1;
+    p.row_parts = static_cast<int>(std::min<int64_t>((p.chunk + blocks - 1) / blocks, rounds));  // about
     parts = static_cast<size_t>(grid) * FEW_ROWS;
     p.seq_bytes = p.n_splits > 1 || kv.weight ? round16(bt.n_seq * sizeof(int2)) : 0;
   } else {
     const PromptSplit split = prompt_split(kv_type, io_type, kv.hd, rl);
     const int64_t want = std::max<int64_t>(1, static_cast<int64_t>(split.per_cu) * n_cu / blocks);
     p.chunk = static_cast<int>((std::max<int64_t>((span + want - 1) / want, split.least) + 63) / 64 * 64);
-    p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
+    p.row_parts = p.n_splits = static_cast<int>((span + p.chunk - 1) / p.chunk);
     parts = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads * p.n_splits;
   }
   const size_t all_rows = static_cast<size_t>(bt.n_seq) * bt.max_new * n_heads;
@@ -793,13 +799,15 @@ int slices_of(int most, int per_cu, const PagedCall& a, int n_cu) {
 // What follows the main kernel: the join where rows are in parts, the weights' sum
 // where the scores were kept.
 template <typename TI, int DP>
-hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
+hipError_t finish(const PagedCall& a, const Plan& p, int n_cu, hipStream_t s) {
   constexpr int LP = DP / 4, MOST = 256 / LP;
   const int items = a.bt.max_new * a.n_heads, groups = a.n_splits > 1 ? (items + MOST - 1) / MOST : 0;
-  // rows side by side where that leaves a work group per CU, else their partials
-  const bool side = static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu;
+  // rows side by side in a work group where they have few partials or fill the CUs so (48
+  // caches in 3 each: 87 us of the call, 90 else), a row's partials where they are many
+  // (two of 100,003 in 64 each: 51 us, 80 side by side)
+  const bool side = p.row_parts <= 4 || static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu;
   const int joins = a.n_splits == 1 ? 0 : side ? groups : items;
-  if (!few) {
+  if (!p.few) {
     if (side) hipLaunchKernelGGL((k_attention_join<TI, DP, MOST>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((k_attention_join<TI, DP, 1>), dim3(joins, a.bt.n_seq), dim3(256), 0, s, a);
   } else {
@@ -811,8 +819,8 @@ hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
   return hipGetLastError();
 }
 template <typename TI>
-hipError_t finish(const PagedCall& a, bool few, int n_cu, hipStream_t s) {
-  return a.kv.hd <= 64 ? finish<TI, 64>(a, few, n_cu, s) : a.kv.hd <= 128 ? finish<TI, 128>(a, few, n_cu, s) : finish<TI, 256>(a, few, n_cu, s);
+hipError_t finish(const PagedCall& a, const Plan& p, int n_cu, hipStream_t s) {
+  return a.kv.hd <= 64 ? finish<TI, 64>(a, p, n_cu, s) : a.kv.hd <= 128 ? finish<TI, 128>(a, p, n_cu, s) : finish<TI, 256>(a, p, n_cu, s);
 }
 
 template <typename TC, typename TI, int DP>
@@ -854,7 +862,7 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
   hipError_t e = p.few ? launch_attention_few(a, p, kv_type, io_type, s) : launch_attention_prompt(a, kv_type, io_type, s);
   if (e != hipSuccess) return e;
   if (p.n_splits > 1 || a.scores) {
-    e = io_type == MCPM_TYPE_F32 ? finish<float>(a, p.few, n_cu, s) : io_type == MCPM_TYPE_F16 ? finish<_Float16>(a, p.few, n_cu, s) : finish<__bf16>(a, p.few, n_cu, s);
+    e = io_type == MCPM_TYPE_F32 ? finish<float>(a, p, n_cu, s) : io_type == MCPM_TYPE_F16 ? finish<_Float16>(a, p, n_cu, s) : finish<__bf16>(a, p, n_cu, s);
     if (e != hipSuccess) return e;
   }
   if (!kv.weight || a.scores || !p.score_len) return hipSuccess;
