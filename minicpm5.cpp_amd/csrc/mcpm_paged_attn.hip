@@ -566,11 +566,12 @@ __device__ __forceinline__ void add_weights(const PagedCall& a, const KeyRange& 
   f32x4 sum{0, 0, 0, 0};
   for (int r0 = 0; r0 < rows; r0 += FEW_ROWS) {
     constexpr int AT_ONCE = 4;  // rows whose scores are asked for together
+    const f32x4 none = f32x4{0, 0, 0, 0} - __builtin_inff();  // no row: share 0
     f32x4 s[AT_ONCE];
     auto ask = [&](int i0) {
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i)
-        s[i] = j < keys.hi && r0 + i0 + i < rows ? *reinterpret_cast<const f32x4*>(sc + static_cast<int64_t>(r0 + i0 + i) * a.score_len) : f32x4{0, 0, 0, 0};
+        s[i] = j < keys.hi && r0 + i0 + i < rows ? *reinterpret_cast<const f32x4*>(sc + static_cast<int64_t>(r0 + i0 + i) * a.score_len) : none;
     };
     ask(0);
     float2 mz = make_float2(MAX_START, 0.0f);
@@ -587,7 +588,7 @@ __device__ __forceinline__ void add_weights(const PagedCall& a, const KeyRange& 
       if (i0) ask(i0);
 #pragma unroll
       for (int i = 0; i < AT_ONCE; ++i) {
-        const float2 f = s_mz[i0 + i];  // past the last row: 1 / z is 0
+        const float2 f = s_mz[i0 + i];
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] += j + k >= keys.lo && j + k < keys.hi ? __builtin_amdgcn_exp2f(s[i][k] - f.x) * f.y : 0.0f;
       }

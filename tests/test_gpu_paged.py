@@ -147,6 +147,15 @@ def test_decode_long_is_split_and_joined(ctx, t, io):
     check_attention(ctx, "long weights", (8, 2, 64), t, io, [5003, 700], [1, 1], page=64, seed=6, weight=True)
 
 
+@pytest.mark.parametrize("t,io", TYPES, ids=IDS)
+@pytest.mark.parametrize("heads", sorted(HEADS))
+def test_decode_weights(ctx, heads, t, io):
+    """The weights that groups of any number of heads add, for one token and a few."""
+    check_attention(ctx, heads, HEADS[heads], t, io, [1, 65, 300], [1, 1, 1], rules=dict(softcap=30.0), weight=True, seed=21)
+    if HEADS[heads][0] // HEADS[heads][1] * 3 <= 32:
+        check_attention(ctx, heads, HEADS[heads], t, io, [70, 400], [3, 2], weight=True, seed=22)
+
+
 @pytest.mark.parametrize("new", [2, 3, 4, 5, 16, 17])
 def test_a_few_tokens_at_once(ctx, new):
     for t, io in ((F32, F32), (F16, F32), (BF16, BF16)):
