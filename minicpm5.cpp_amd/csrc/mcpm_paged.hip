@@ -228,7 +228,11 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView b
   const int j0 = begin + tid * V;
   unsigned key[V];
   load_keys<V>(kv, bt, b, h, j0, end, key);
-  auto candidate = [&](int i) { return j0 + i >= first && j0 + i < end; };
+  // bit i: position i of the lane's is a candidate (bits, for V conditions held through the
+  // passes would fill the scalar registers)
+  unsigned cand = ((1u << min(max(end - j0, 0), V)) - 1) & ~((1u << min(max(first - j0, 0), V)) - 1);
+  auto candidate = [&](int i) { return (cand >> i & 1) != 0; };
+  auto held = [&] { asm volatile("" : "+v"(cand)); };
   unsigned edge = 0;
   int need = budget - first - recent;
 #pragma unroll 1
@@ -237,6 +241,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView b
     const unsigned mask = pass == 0 ? 0u : pass == 1 ? ~0u << 21 : ~0u << 10;
     for (int i = tid; i < EV_BINS; i += EV_T) hist[i] = 0;
     __syncthreads();
+    held();
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (candidate(i) && (key[i] & mask) == edge) atomicAdd(&hist[(key[i] >> shift) & (bins - 1)], 1);
@@ -245,6 +250,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView b
     edge |= static_cast<unsigned>(s_edge.bin) << shift;
     need = s_edge.need;
   }
+  held();
   unsigned keep = 0;  // bit i: position i of the lane's is kept
   int n[1] = {0}, all[1];
   if (s_edge.count != need) {  // the first `need` of the equal ones
@@ -255,6 +261,7 @@ __global__ void __launch_bounds__(EV_T) k_evict_select(PagedView kv, BatchView b
     need = INT_MAX;
   }
   int rank = n[0];
+  held();
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (candidate(i) && (key[i] > edge || (key[i] == edge && rank++ < need))) keep |= 1u << i;

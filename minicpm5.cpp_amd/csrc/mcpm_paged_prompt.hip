@@ -430,7 +430,8 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
   for (int seg = c0; seg < c1; seg += SEG) {
     const int seg_end = min(c1, seg + SEG);
     __syncthreads();
-    const bool ok = load_page_offsets(a.bt, kv, b, seg, seg_end, s_off);
+    const PagedCall& again = call_again();
+    const bool ok = load_page_offsets(again.bt, again.kv, b, seg, seg_end, s_off);
     const int n_tiles = (seg_end - seg + KT - 1) / KT;
     if (tid == 0) s_tiles = docs ? 0u : n_tiles == 32 ? ~0u : (1u << n_tiles) - 1;
     const bool bad_pages = __syncthreads_or(!ok);
@@ -464,7 +465,8 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
     const bool tagged = docs || bad_pages;
     auto stage_tags = [&](int at, int p0) {
       if (!tagged || wv) return;
-      const int tag = lane < KT ? tag_of(a.rl, a.bt, kv, b, min(p0 + lane, seg_end - 1), bad_pages) : s_tags[0];
+      const PagedCall& c = call_again();
+      const int tag = lane < KT ? tag_of(c.rl, c.bt, c.kv, b, min(p0 + lane, seg_end - 1), bad_pages) : s_tags[0];
       if (lane < KT) s_tag[at][lane] = tag;
       const bool plain = !__any(tag != s_tags[0]);
       if (lane == 0) s_plain[at] = plain;
@@ -558,22 +560,23 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
   }
 
   z += lane_xor32(z);
-  const bool final = a.n_splits == 1;
+  const PagedCall& c = call_again();
+  const bool final = c.n_splits == 1;
   const float inv = z == 0.0f ? 0.0f : 1.0f / z;
-  const int64_t at = part_index(a, b, t, head, split);
+  const int64_t at = part_index(c, b, t, head, split);
   bool bad = false;
   if (row_in) {
     bad = !(z < __builtin_inff());
-    TI* dst = static_cast<TI*>(a.out) + row * a.out_stride + head * kv.hd;
-    float* part = a.part_o + at * kv.hd;
+    TI* dst = static_cast<TI*>(c.out) + row * c.out_stride + head * c.kv.hd;
+    float* part = c.part_o + at * c.kv.hd;
 #pragma unroll
-    for (int c = 0; c < Tile::RUNS; ++c) {
-      const int d = Tile::run_at(c);
-      if (d < kv.hd) {
+    for (int u = 0; u < Tile::RUNS; ++u) {
+      const int d = Tile::run_at(u);
+      if (d < c.kv.hd) {
         float x[Tile::RUN];
 #pragma unroll
         for (int i = 0; i < Tile::RUN; ++i) {
-          x[i] = tile.run(c, i);
+          x[i] = tile.run(u, i);
           bad = bad || x[i] - x[i] != 0.0f;
         }
 #pragma unroll
@@ -591,8 +594,8 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
       }
     }
     if (half == 0) {
-      if (a.part_mz) a.part_mz[at] = make_float2(m, z);
-      if (final && a.row_mz) a.row_mz[row_index(a, b, t, head)] = make_float2(m, z);
+      if (c.part_mz) c.part_mz[at] = make_float2(m, z);
+      if (final && c.row_mz) c.row_mz[row_index(c, b, t, head)] = make_float2(m, z);
     }
   }
   if (!__syncthreads_or(bad)) return;
@@ -603,7 +606,7 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
   __syncthreads();
   float* lds = reinterpret_cast<float*>(s_tile[0]);
   exact_rows<TC, TI>(b, kh, rb, PR_ROWS, c0, c1, final, s_bad, lds, lds + PAGED_MAX_HD, lds + 2 * PAGED_MAX_HD,
-                     [&](const PagedCall& c, int, int tt, int h) { return part_index(c, b, tt, h, split); });
+                     [&](const PagedCall& x, int, int tt, int h) { return part_index(x, b, tt, h, split); });
 }
 
 template <typename TC, typename TI, int DP>

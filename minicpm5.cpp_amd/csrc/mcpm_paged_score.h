@@ -205,9 +205,10 @@ __device__ __forceinline__ bool load_page_offsets(const BatchView& bt, const Pag
 // The call's own copy in the kernel's arguments: what the rare ends of a kernel need
 // is read again there rather than held in scalar registers through its loops.
 __device__ __forceinline__ const PagedCall& call_again() {
-  const void* p = (const void*)__builtin_amdgcn_kernarg_segment_ptr();
+  // in the constant address space until the last cast: the loads stay scalar
+  const __attribute__((address_space(4))) void* p = (const __attribute__((address_space(4))) void*)__builtin_amdgcn_kernarg_segment_ptr();
   asm volatile("" : "+s"(p));
-  return *static_cast<const PagedCall*>(p);
+  return *(const PagedCall*)p;
 }
 
 // The plain computation of one row over positions [c0, c1), by the whole work
