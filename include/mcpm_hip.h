@@ -228,7 +228,9 @@ typedef struct {
  * sequence is taken as one of max_len (or of the positions its table holds),
  * rows past max_new are left out, and a page number outside the pool's holds
  * nothing (a position there is neither stored nor seen).  A row whose position
- * would be negative sees nothing and is not stored. */
+ * would be negative sees nothing and is not stored.  A page that a table lists
+ * twice is read as often; where a call writes (append, weights), its positions
+ * then race. */
 typedef struct {
     int n_seq, n_rows;
     int max_new, max_len, max_pages;
@@ -282,10 +284,11 @@ int mcpm_paged_attention(mcpm_ctx *ctx, void *out, int64_t out_stride, const voi
  * (equal ones: the lowest position; NaN counts as less than any), and copies what
  * is kept, k, v and weight, in order, to positions 0.. of dst_pages (int
  * [n_seq][max_dst_pages], pages of the same pool that no sequence of the call
- * uses).  kept (int [n_seq][n_kv_heads][budget]): the positions they had, -1 past
+ * uses; dst_pages and dst_lens are memory of their own).  kept (int [n_seq][n_kv_heads][budget]): the positions they had, -1 past
  * dst_lens[b] = min(lens[b], budget).  kv->weight is required; batch's rows
  * (starts, n_rows, max_new) are not read.  Kept keys stay rotated by the position
- * they had. */
+ * they had.  Past 16,384 candidates the scratch is 9 bytes for each position up to
+ * max_len of every sequence and kv head. */
 int mcpm_paged_evict(mcpm_ctx *ctx, const mcpm_paged_kv *kv, const mcpm_paged_batch *batch, int budget, int first,
                      int recent, const int *dst_pages, int max_dst_pages, int *kept, int *dst_lens);
 

@@ -135,11 +135,16 @@ int mcpm_paged_attention(mcpm_ctx* c, void* out, int64_t out_stride, const void*
     rc = fail(MCPM_ERR_ARG, std::string(fn) + ": n_heads must be a multiple of n_kv_heads");
   if (!rc) rc = check_rows(q, q_stride, n_heads, kv->head_dim, io_type, fn, "q");
   if (!rc) rc = check_rows(out, out_stride, n_heads, kv->head_dim, io_type, fn, "out");
+  if (!rc && static_cast<int64_t>(bt.max_new) * n_heads > INT32_MAX)
+    rc = fail(MCPM_ERR_ARG, std::string(fn) + ": max_new * n_heads must be less than 2^31");
   if (rc) return rc;
   RuleView rl{};
   if (rules) {
-    if (!std::isfinite(rules->scale) || !(rules->softcap >= 0.0f && std::isfinite(rules->softcap)) || rules->window < 0)
-      return fail(MCPM_ERR_ARG, std::string(fn) + ": scale must be finite, softcap and window not negative");
+    constexpr float most = 1e38f;  // times log2(e) still finite
+    if (!(std::fabs(rules->scale) <= most) || !(rules->softcap >= 0.0f && rules->softcap <= most) || rules->window < 0)
+      return fail(MCPM_ERR_ARG, std::string(fn) + ": scale must be finite, softcap and window not negative, none past 1e38");
+    if (rules->softcap > 0.0f && !(std::fabs(rules->scale / rules->softcap) <= most))
+      return fail(MCPM_ERR_ARG, std::string(fn) + ": scale / softcap must not be past 1e38");
     if (rules->docs && rules->docs_stride < bt.max_len)
       return fail(MCPM_ERR_ARG, std::string(fn) + ": docs_stride is less than max_len");
     rl = RuleView{rules->scale, rules->softcap, rules->window, rules->slopes, rules->prefix, rules->docs, rules->docs_stride};

@@ -513,6 +513,16 @@ __global__ void __launch_bounds__(256, (prompt_waves<TC, TI, DP>())) k_attention
 #pragma unroll
         for (int j = 0; j < Tile::NO; ++j) tile.o[j] *= f;
       }
+      // The shares take s * scale - m with one rounding.  Beyond 2^24 that difference holds
+      // the rounding of m, whole units there: the scores are rounded as m was first.
+      if (__any(fabsf(m) > 16777216.0f && m > MAX_START)) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          asm volatile("" : "+v"(s[i]));
+          s[i] *= scale;
+        }
+        scale = 1.0f;
+      }
       return scale;
     };
     int cur = __builtin_ctz(todo), buf = 0;

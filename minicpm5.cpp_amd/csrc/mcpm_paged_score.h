@@ -10,8 +10,9 @@ namespace mcpm {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 // The running maximum's start: finite, so that what is not seen (a score of
-// -inf) has share 0 and a NaN stays one.
-constexpr float MAX_START = -1e30f;
+// -inf) has share 0 and a NaN stays one, and below the scores that 32 bits hold
+// but for the last bit of their exponent.
+constexpr float MAX_START = -3e38f;
 
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));

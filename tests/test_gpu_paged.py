@@ -433,6 +433,33 @@ def test_large_scores(ctx, t, io, new):
     assert np.isfinite(got).all() and (np.abs(got - want) <= bound).all()
 
 
+@pytest.mark.parametrize("t,io", [(F32, F32), (BF16, F32), (BF16, BF16)], ids=["f32-f32", "bf16-f32", "bf16-bf16"])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_far_below_zero(ctx, t, io, new):
+    """Equal scores of -3e32: every seen position has the same share, however low the scores are."""
+    H, KH, hd, n = 4, 1, 8, 300
+    rng = np.random.default_rng(23)
+    cache = R.Cache(t, 20, 16, KH, hd, rng=rng, weight=True)
+    cache.k[:] = R.store(np.full(cache.k.shape, -1e16), t)
+    cache.weight[:] = 0.0
+    tables = tables_of(rng, [n], 16, 20)
+    q = R.store(np.full((new, H * hd), 1e16), io)
+    announce(f"far below zero {NAME[t]}/{NAME[io]} new={new}")
+    dev = Dev(ctx, cache, tables, [n], [new])
+    got = run_attention(ctx, dev, q, io, H, {})
+    v = np.stack([R.load(cache.v, t).reshape(-1)[cache.index(tables[0][j // 16], j % 16, 0)] for j in range(n)])
+    eps = 2.0 ** -24 if io == F32 else 2.0 ** -8
+    w = np.zeros(n)
+    for r in range(new):
+        seen = n - new + r + 1
+        w[:seen] += H / seen
+        want, size = v[:seen].astype(np.float64).mean(0), np.abs(v[:seen]).astype(np.float64).mean(0)
+        # shares of exactly 1 to be summed and divided by; the output rounded once
+        assert (np.abs(got[r] - want) <= (seen + 4) * 2.0 ** -24 * size + eps * np.abs(want)).all()
+    got_w = np.array([dev.image("weight")[tables[0][j // 16], 0, j % 16] for j in range(n)])
+    assert (np.abs(got_w - w) <= (new * H + 4) * 2.0 ** -23 * w).all()
+
+
 def test_f32_rows_beyond_half_range(ctx):
     """F32 rows whose values pass a half's range, and tiny ones, over F16 and BF16 caches."""
     H, KH, hd, n = 4, 2, 64, 80

@@ -51,6 +51,15 @@ def accepted(lib, rc):
     refused(lib, rc, mcpm.ERR_ARG, "null context")
 
 
+def test_values_past_the_range_are_refused(lib):
+    for rules in (mcpm.AttnRules(scale=2e38), mcpm.AttnRules(scale=-2e38), mcpm.AttnRules(softcap=2e38),
+                  mcpm.AttnRules(scale=1e10, softcap=1e-30), mcpm.AttnRules(scale=float("nan"))):
+        refused(lib, attention(lib, rules=rules), mcpm.ERR_ARG, "1e38")
+    accepted(lib, attention(lib, rules=mcpm.AttnRules(scale=1e37, softcap=1e38)))
+    many = batch(n_rows=1 << 30, max_new=1 << 30)
+    refused(lib, attention(lib, batch_=many), mcpm.ERR_ARG, "max_new * n_heads")
+
+
 def test_sound_calls_get_as_far_as_the_context(lib):
     for rc in (attention(lib), append(lib), evict(lib), logits(lib)):
         accepted(lib, rc)
