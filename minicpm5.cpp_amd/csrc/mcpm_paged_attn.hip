@@ -29,7 +29,7 @@ namespace {
 // Bound by the bytes of the cache, each read once: two caches of 100,003 positions x 2
 // bfloat16 heads of 128, 205 MB, take 43 us (4.8 TB/s, what a large copy reaches) and 7.5
 // to join; 48 ragged ones of up to 4099 x 8 heads of 64 halves for 32-bit rows, 251 MB,
-// 72 us (3.5 TB/s: work groups of unequal ends, two terms, a capped score and its store)
+// 68 us (3.7 TB/s: work groups of unequal ends, two terms, a capped score and its store)
 // and 12.5 to join and weigh; one of 513 x 8 heads of 64, 32 bits, 8.5 us, a chain of
 // dependent loads (lengths, pages, rows), and 3.1.
 
@@ -233,9 +233,12 @@ __host__ __device__ inline int few_max_rounds(const PagedView& kv) { return FEW_
 // Which part of which sequence this work group has.  The host knows a bound of the
 // lengths only, and they are ragged: every work group sums up the rounds of all
 // sequences and takes its share of them, the same number of rounds (the last of a
-// sequence fewer).  A block's chunks are `stride` work groups apart.
+// sequence fewer).  Its number is its block index or, with by_xcd (up to 256 sequences),
+// counts along the XCDs, so that the heads of a page are read through one L2 and its
+// translations (48 ragged caches of 8 heads of 64: 82 us of the call, 87 without; with
+// one work group per CU the XCDs' shares are too unequal, 75 us for 65).
 struct Share {
-  int b, chunk, n_chunks, kh, rb, rounds, first;
+  int b, chunk, n_chunks, kh, rb, rounds, first, id;
 };
 __device__ __forceinline__ bool few_share(const PagedCall& a, Share* s_share, int64_t (*s_wave)[4], Share& out) {
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, per = a.kv.n_kv_heads, n = a.bt.n_seq;
@@ -266,10 +269,16 @@ __device__ __forceinline__ bool few_share(const PagedCall& a, Share* s_share, in
     if (lane == 63) s_wave[1][wv] = x;
     __syncthreads();
     for (int i = 0; i < 4; ++i) x += i < wv ? s_wave[1][i] : 0;
-    const int64_t first = base + x - mine, i = static_cast<int64_t>(blockIdx.x) - first;
+    const int64_t first = base + x - mine;
+    int64_t id = blockIdx.x;
+    if (a.by_xcd) {
+      const int64_t per_xcd = (s_wave[1][0] + s_wave[1][1] + s_wave[1][2] + s_wave[1][3]) / 8;
+      if (id < per_xcd * 8) id = id % 8 * per_xcd + id / 8;
+    }
+    const int64_t i = id - first;
     if (i >= 0 && i < mine) {
       const int k = static_cast<int>(i), pairs = w.blocks * per;
-      *s_share = Share{b, k / pairs, chunks, k % per, k % pairs / per, rounds, static_cast<int>(first)};
+      *s_share = Share{b, k / pairs, chunks, k % per, k % pairs / per, rounds, static_cast<int>(first), static_cast<int>(id)};
     }
     base += s_wave[1][0] + s_wave[1][1] + s_wave[1][2] + s_wave[1][3];
   }
@@ -282,6 +291,7 @@ __device__ __forceinline__ bool few_share(const PagedCall& a, Share* s_share, in
   out.rb = __builtin_amdgcn_readfirstlane(out.rb);
   out.rounds = __builtin_amdgcn_readfirstlane(out.rounds);
   out.first = __builtin_amdgcn_readfirstlane(out.first);
+  out.id = __builtin_amdgcn_readfirstlane(out.id);
   return out.b >= 0;
 }
 
@@ -304,7 +314,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   const KeyRange keys = key_range(a.rl, b, fb.pos0, fb.pos0 + sr.n - 1, len);
   const int c0 = keys.lo + sh.chunk * sh.rounds * FEW_ROUND, c1 = min(keys.hi, c0 + sh.rounds * FEW_ROUND);
   const bool final = sh.n_chunks == 1;
-  if (static_cast<int>(blockIdx.x) == sh.first && tid == 0 && a.seq_wgs) a.seq_wgs[b] = make_int2(sh.first, sh.n_chunks);
+  if (sh.id == sh.first && tid == 0 && a.seq_wgs) a.seq_wgs[b] = make_int2(sh.first, sh.n_chunks);
 
   const int r = rb * FEW_ROWS + n16;
   const bool row_in = r < fb.r_end;
@@ -443,7 +453,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
     Z += w[i] * s_z[i][rn];
   }
   const int64_t rowj = sr.r0 + tj;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * FEW_ROWS + rn;
+  const int64_t at = static_cast<int64_t>(sh.id) * FEW_ROWS + rn;
   const float inv = Z == 0.0f ? 0.0f : 1.0f / Z;
   TI* dst = static_cast<TI*>(a.out) + rowj * a.out_stride + hj * kv.hd;
   bool bad = !(Z < __builtin_inff());
@@ -473,7 +483,7 @@ __global__ void __launch_bounds__(256) k_attention_few(const PagedCall a) {
   if (!s_bad) return;
   // Something infinite or NaN came up: perhaps only a share of 0 times it.
   exact_rows<TC, TI>(b, kh, rb, FEW_ROWS, c0, c1, final, nullptr, &s_o[0][0][0], &s_o[2][0][0], &s_m[0][0],
-                     [](const PagedCall&, int i, int, int) { return static_cast<int64_t>(blockIdx.x) * FEW_ROWS + i; });
+                     [&](const PagedCall&, int i, int, int) { return static_cast<int64_t>(sh.id) * FEW_ROWS + i; });
 }
 
 // Where a row's partials are: n of them, `stride` apart.
@@ -702,7 +712,7 @@ __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
 // How a call is cut into work groups.  Up to FEW_MOST rows of a sequence and kv
 // head take the 16-row kernel, more the prompt kernel.
 struct Plan {
-  bool few;
+  bool few, by_xcd;
   int block_rows, n_blocks, chunk, n_splits, grid, lds_pages, row_parts, score_len;
   size_t o_bytes, mz_bytes, row_bytes, seq_bytes, score_bytes;
   size_t bytes() const { return o_bytes + mz_bytes + row_bytes + seq_bytes + score_bytes; }
@@ -749,8 +759,10 @@ Plan plan_of(const PagedView& kv, int kv_type, const BatchView& bt, const RuleVi
     // One work group per CU keeps its memory busy, and more of them start later (two
     // caches of 100,003, heads of 128: 50 us, 61 with two).  Heads of up to 64 leave room
     // for more at once, which evens out many ragged sequences of costly rules (48 with
-    // weights and a cap: 90 us instead of 97; a single one of 40,000 loses, 33 for 25).
-    const int per_cu = kv.hd <= 64 && blocks >= n_cu ? FEW_TARGET_64 : FEW_TARGET;
+    // weights and a cap: 82 us instead of 97; a single one of 40,000 loses, 33 for 25).
+    const bool many = kv.hd <= 64 && blocks >= n_cu;
+    const int per_cu = many ? FEW_TARGET_64 : FEW_TARGET;
+    p.by_xcd = many && bt.n_seq <= 256;
     p.chunk = per_cu * n_cu;
     // few_share gives a block a work group more than its share, at most, and none more than max_rounds
     const int max_rounds = few_max_rounds(kv);
@@ -811,7 +823,7 @@ hipError_t finish(const PagedCall& a, const Plan& p, int n_cu, hipStream_t s) {
   constexpr int LP = DP / 4, MOST = 256 / LP;
   const int items = a.bt.max_new * a.n_heads, groups = a.n_splits > 1 ? (items + MOST - 1) / MOST : 0;
   // rows side by side in a work group where they have few partials or fill the CUs so (48
-  // caches in 3 each: 87 us of the call, 90 else), a row's partials where they are many
+  // caches in 3 each save 3 us of the call), a row's partials where they are many
   // (two of 100,003 in 64 each: 51 us, 80 side by side)
   const bool side = p.row_parts <= 4 || static_cast<int64_t>(items) * a.bt.n_seq >= static_cast<int64_t>(MOST) * n_cu;
   const int joins = a.n_splits == 1 ? 0 : side ? groups : items;
@@ -859,7 +871,7 @@ hipError_t launch_paged_attention(const PagedView& kv, int kv_type, const BatchV
     sc += bytes;
     return at;
   };
-  PagedCall a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.block_rows, p.n_blocks, p.chunk, p.n_splits};
+  PagedCall a{kv, bt, rl, q, out, q_stride, out_stride, n_heads, group, p.block_rows, p.n_blocks, p.chunk, p.n_splits, p.by_xcd};
   a.part_o = reinterpret_cast<float*>(take(p.o_bytes));
   a.part_mz = reinterpret_cast<float2*>(take(p.mz_bytes));
   a.row_mz = reinterpret_cast<float2*>(take(p.row_bytes));

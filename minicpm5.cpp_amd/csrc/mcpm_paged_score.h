@@ -160,6 +160,7 @@ struct PagedCall {
   int64_t q_stride, out_stride;
   int n_heads, group, block_rows, n_blocks;  // query heads per kv head; row blocks per (sequence, kv head)
   int chunk, n_splits;  // few rows: work groups wanted, and whether there can be more than one to a block
+  bool by_xcd;          // few rows: consecutive parts of the work on one XCD
   float* part_o;    // unnormalised: [seq][new token][head][split][hd]; few rows: [work group][row of the block][hd]
   float2* part_mz;  // the same without [hd]
   float2* row_mz;   // [seq][new token][head]: the rows' own, with weights

@@ -156,6 +156,16 @@ def test_decode_weights(ctx, heads, t, io):
         check_attention(ctx, heads, HEADS[heads], t, io, [70, 400], [3, 2], weight=True, seed=22)
 
 
+@pytest.mark.parametrize("n_seq", [40, 256, 257, 300])
+def test_many_ragged_sequences(ctx, n_seq):
+    """More (sequence, kv head) pairs than CUs, lengths from 0 on, some sequences in several parts."""
+    rng = np.random.default_rng(24)
+    lens = [int(n) for n in rng.integers(0, 60, n_seq)]
+    lens[3], lens[n_seq - 2] = 2500, 1300
+    for t, io in ((F16, F32), (BF16, BF16)):
+        check_attention(ctx, "many", (8, 8, 16), t, io, lens, [1] * n_seq, page=64, weight=True, seed=25)
+
+
 @pytest.mark.parametrize("new", [2, 3, 4, 5, 16, 17])
 def test_a_few_tokens_at_once(ctx, new):
     for t, io in ((F32, F32), (F16, F32), (BF16, BF16)):
