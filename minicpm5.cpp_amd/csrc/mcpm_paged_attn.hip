@@ -724,18 +724,18 @@ constexpr size_t MOST_SCORES = size_t{1} << 30;  // bytes of kept scores, past w
 // split pays for its join where a tile of keys is dear: on the 32-bit matrix
 // instructions, 1/8 of the rate, anywhere (heads of 256, 200 tokens: 82 us whole, 48 in
 // chunks of 64), there with four work groups per CU, which even out the causal triangle
-// (heads of 128, 2400 tokens: 381 us with one, 240 with four; under a window, which has
-// no triangle, one: 164 us, 242 with four); with heads of 256 or 32-bit rows over a
+// (heads of 128, 2400 tokens: 381 us with one, 240 with four; under a window or with
+// documents, which leave no triangle, one: 164 us, 242 with four); with heads of 256 or 32-bit rows over a
 // 16-bit cache's heads of 128 in chunks of 128 (1000 tokens, 8 heads of 256: 124 us
 // whole, 82 split); not elsewhere (300 tokens, heads of 64: 12 us whole, 15 split), nor
-// where documents leave most of a chunk unseen (260 tokens in documents of 30, heads of
-// 256: 38 us whole, 44 split).
+// over 16 bits where documents leave most of a chunk unseen (260 tokens in documents of
+// 30, heads of 256: 38 us whole, 44 split).
 struct PromptSplit {
   int per_cu, least;
 };
 PromptSplit prompt_split(int kv_type, int io_type, int hd, const RuleView& rl) {
+  if (kv_type == MCPM_TYPE_F32) return {rl.docs || (rl.window > 0 && !rl.prefix) ? 1 : 4, 64};
   if (rl.docs) return {1, 512};
-  if (kv_type == MCPM_TYPE_F32) return {rl.window > 0 && !rl.prefix ? 1 : 4, 64};
   return {1, hd > 128 || (hd > 64 && io_type == MCPM_TYPE_F32) ? 128 : 512};
 }
 

@@ -68,11 +68,11 @@ __device__ __forceinline__ float tanh_small(float x) {
   p = __builtin_fmaf(p, x2, -3.3333333333e-1f);
   return __builtin_fmaf(x * x2, p, x);
 }
-// Above from exp(2x).
+// Above from exp(-2x) as (1 - e) / (1 + e), whose numerator is exact where it is small.
 __device__ __forceinline__ float tanh_f32(float x) {
   const float a = fabsf(x);
-  const float e = __builtin_amdgcn_exp2f(a * (2.0f * LOG2E));
-  const float large = 1.0f - 2.0f * __builtin_amdgcn_rcpf(e + 1.0f);
+  const float e = __builtin_amdgcn_exp2f(a * (-2.0f * LOG2E));
+  const float large = (1.0f - e) * __builtin_amdgcn_rcpf(1.0f + e);
   return a < TANH_SERIES ? tanh_small(x) : __builtin_copysignf(large, x);
 }
 
