@@ -668,6 +668,7 @@ __device__ __forceinline__ void weights_again(const PagedCall& a, int p0, int kh
     const float inv = in && mz.y != 0.0f ? 1.0f / mz.y : 0.0f;
     const RowRule rr = row_rule(a.rl, b, in ? pos : -1, len);
     const float slope = a.rl.slopes ? a.rl.slopes[head] * LOG2E : 0.0f;
+    const int j0 = p0 + 4 * g;
     Tile tile;
     tile.load_q(static_cast<const TI*>(a.q) + (sr.r0 + t) * a.q_stride + head * kv.hd, kv.hd, rule.mul);
 #pragma unroll
@@ -682,7 +683,7 @@ __device__ __forceinline__ void weights_again(const PagedCall& a, int p0, int kh
       scores_of<8>(rule, s, tile.mul);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int j = p0 + 32 * n + 16 * (i >> 2) + 4 * g + (i & 3);
+        const int j = j0 + 32 * n + 16 * (i >> 2) + (i & 3);
         const float x = s[i] - slope * fabsf(static_cast<float>(pos - j));
         sum[n][i] += in_span(rr, j) && tag[n][i] == rr.tag ? __builtin_amdgcn_exp2f(x - mz.x) * inv : 0.0f;
       }
@@ -706,7 +707,7 @@ __device__ __forceinline__ void weights_again(const PagedCall& a, int p0, int kh
 template <typename TC, typename TI, int DP>
 __global__ void __launch_bounds__(256) k_prompt_weight(const PagedCall a) {
   const int len = seq_len(a.bt, a.kv, blockIdx.z);
-  for (int p0 = blockIdx.x * WEIGHT_KEYS; p0 < len; p0 += gridDim.x * WEIGHT_KEYS) weights_again<TC, TI, DP>(a, p0, blockIdx.y, blockIdx.z);
+  for (int p0 = blockIdx.x * WEIGHT_KEYS; p0 < len; p0 += gridDim.x * WEIGHT_KEYS) weights_again<TC, TI, DP>(call_again(), p0, blockIdx.y, blockIdx.z);
 }
 
 // How a call is cut into work groups.  Up to FEW_MOST rows of a sequence and kv
