@@ -274,7 +274,9 @@ int mcpm_paged_append(mcpm_ctx *ctx, const mcpm_paged_kv *kv, const mcpm_paged_b
  * are not rounded to 16 bits.  With kv->weight, each seen position's weight grows
  * by its share p (they sum to 1 per row and head), summed over the kv head's
  * query heads and the rows, in an order that does not change from call to call;
- * sequences that share a page then race. */
+ * sequences that share a page then race.  A prompt's weights come from scores
+ * formed a second time: scores past 2^20, whose last bits decide a share, may
+ * weigh otherwise than they were summed in out. */
 int mcpm_paged_attention(mcpm_ctx *ctx, void *out, int64_t out_stride, const void *q, int64_t q_stride, int io_type,
                          int n_heads, const mcpm_paged_kv *kv, const mcpm_paged_batch *batch,
                          const mcpm_attn_rules *rules);
